@@ -374,6 +374,100 @@ int pse_rope(void *qkv, int64_t ld, int32_t rows, int32_t width, int32_t q_heads
 int pse_rope_pos(void *qkv, int64_t ld, int32_t rows, int32_t width, int32_t q_heads, int32_t kv_heads,
                  int32_t head_dim, const int32_t *positions, float theta, int32_t dtype, void *stream);
 
+/* Rotary positions.  Pair i of the first rotary_dim elements of a head turns
+ * by positions[t] * turns[i] turns (turns[i] = f_i / 2 pi in fp64, rotary_dim /
+ * 2 entries on the device): y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin, both
+ * times `factor`; pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) if
+ * interleaved; the rest of the head is copied.  head_dim and rotary_dim are
+ * even.  A position is any int32.  No counterpart in the reference, whose
+ * positions are learned (engine/model.py:174-181). */
+typedef struct {
+  const double *turns;
+  float factor;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t interleaved;
+} pse_rotary_spec;
+
+/* [tokens, heads, head_dim] with element strides; a head's elements are
+ * contiguous. */
+typedef struct {
+  void *data;
+  int64_t tok_stride;
+  int64_t head_stride;
+  int32_t heads;
+} pse_head_view;
+
+/* q -> q_out and k -> k_out (either may have 0 heads); out may be the input
+ * itself, but must not overlap it otherwise. */
+int pse_rotary(pse_rotary_spec r, pse_head_view q, pse_head_view q_out, pse_head_view k, pse_head_view k_out,
+               const int32_t *positions, int64_t tokens, int32_t dtype, void *stream);
+
+/* pse_rotary with the copy half of PagedKVCache.append
+ * (engine/paged_cache.py:131-136): token t's turned K and its V also go to
+ * position cache_pos[t] of slot slots[t] (blocks reserved before; a token
+ * whose block is not held is dropped, as pse_kv_append drops it).  k_out.data
+ * may be NULL.  The tensors have the pool's dtype. */
+int pse_rotary_append(pse_block_state st, pse_kv_layer kv, pse_rotary_spec r, pse_head_view q, pse_head_view q_out,
+                      pse_head_view k, pse_head_view k_out, pse_head_view v, const int32_t *positions,
+                      const int32_t *slots, const int32_t *cache_pos, int64_t tokens, void *stream);
+
+/* ---- attention over packed prompts ---- */
+
+/* The work list of pse_prompt_attention for `n` prompts of lens[i] >= 0 tokens
+ * (host arrays; nothing is launched).  *n_ints receives the list's size; with
+ * plan != NULL the list is written there (plan_ints >= *n_ints, else
+ * PSE_EWORKSPACE).  n_cta: CTAs the work is dealt to, one per multiprocessor.
+ * The caller copies the list to the device (16-byte aligned) and may use it
+ * for every layer of the forward; its items number (*n_ints - (n_cta + 4) / 4 *
+ * 4) / 4. */
+int pse_prompt_plan(const int32_t *lens, int32_t n, int32_t q_heads, int32_t kv_heads, int32_t n_cta, int32_t *plan,
+                    int64_t plan_ints, int64_t *n_ints);
+
+/* Causal attention of packed prompts (engine/model.py:99-116 without padding):
+ * q, k, v and out are [tokens, heads, head_dim], prompt after prompt as planned;
+ * token i of a prompt attends to tokens 0..i of that prompt, query head h to K/V
+ * head h / (q.heads / k.heads); head_dim <= 256.  A row whose weights sum to
+ * zero gives zero.  bf16 with head_dim 64 or 128, at most 128 heads a group and
+ * 16-byte aligned rows runs on the tensor cores, the rest in fp32 on the CUDA
+ * cores.  Items that lie outside the tensors are skipped.  `status` (nullable)
+ * receives PSE_STATUS_TIMEOUT if a bounded in-kernel wait expires.  `plan` is
+ * the device copy of pse_prompt_plan's list. */
+int pse_prompt_attention(pse_head_view q, pse_head_view k, pse_head_view v, pse_head_view out, int64_t tokens,
+                         int32_t head_dim, int32_t dtype, float scale, const int32_t *plan, int32_t n_cta,
+                         int64_t n_items, int32_t *status, void *stream);
+
+/* ---- attention of token trees of any shape ---- */
+
+/* Ancestor masks and depths of packed trees: parents[node_off[i] + j] is the
+ * parent of row i's node j within the row (< j), or negative for a child of the
+ * root context.  Bit m of node j's `words` 64-bit words: node m is j or an
+ * ancestor of j.  depths: 0 for a child of the root.  A parent that does not
+ * precede its child ends the walk. */
+int pse_tree_masks(const int32_t *parents, const int32_t *node_off, int32_t rows, int32_t n_nodes, int32_t words,
+                   int64_t *masks, int32_t *depths, void *stream);
+
+/* pse_paged_attention for token trees of any shape, ragged over the rows (the
+ * reference lists trees as future work).  Row i's nodes are the queries
+ * node_off[i]..node_off[i+1]-1 of q and out ([n_nodes, heads, head_dim]); node
+ * j's K/V stands in the pool at position ctx[i] + j of slots[i].  Node j
+ * attends to positions 0..ctx[i]-1 and to the row's nodes m whose bit is set in
+ * its mask (`words` 64-bit words per node; bits past the row's nodes are
+ * ignored, and a node need not see itself).  A node that sees nothing gives
+ * zero, as do the nodes of a row with an invalid slot or a context the block
+ * table cannot hold.  max_nodes bounds the rows' node counts (it picks the
+ * kernel's shape; max_nodes <= 64 words).  ctx, slots and node_off are read on
+ * the device only, so the call can be captured and replayed with other values.
+ * workspace: pse_token_tree_workspace() bytes, 16-byte aligned, the first 2048
+ * of them zero before the first call and zero again after every call; calls
+ * that share one must not overlap on the GPU. */
+int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,
+                             const int32_t *slots, const int32_t *ctx, const int32_t *node_off, int32_t rows,
+                             int32_t n_nodes, int32_t max_nodes, const int64_t *masks, int32_t words, float scale,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+size_t pse_token_tree_workspace(int32_t head_dim);
+
 /* Scatter rows: dst[index[i] * ld_dst + :n] = src[i * ld_src + :n] (fp32),
  * for index[i] in [0, n_dst_rows). */
 int pse_scatter_rows(const float *src, int64_t ld_src, const int32_t *index, int32_t rows, int32_t n,

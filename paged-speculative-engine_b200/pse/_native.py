@@ -49,6 +49,14 @@ class KVLayer(ctypes.Structure):
     _fields_ = [("k_pool", c_p), ("v_pool", c_p), ("kv_heads", c_i32), ("head_dim", c_i32), ("dtype", c_i32)]
 
 
+class RotarySpec(ctypes.Structure):
+    _fields_ = [("turns", c_p), ("factor", c_f32), ("head_dim", c_i32), ("rotary_dim", c_i32), ("interleaved", c_i32)]
+
+
+class HeadView(ctypes.Structure):
+    _fields_ = [("data", c_p), ("tok_stride", c_i64), ("head_stride", c_i64), ("heads", c_i32)]
+
+
 # name -> (argtypes, kernels launched per call)
 _PROTOS = {
     "pse_block_init": ([BlockState, c_p], 1),
@@ -79,6 +87,15 @@ _PROTOS = {
                       c_i32, c_p], 1),
     "pse_epilogue": ([c_i32, c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i32, c_i32, c_i32, c_p], 1),
     "pse_rope": ([c_p, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_p, c_f32, c_i32, c_p], 1),
+    "pse_rotary": ([RotarySpec, HeadView, HeadView, HeadView, HeadView, c_p, c_i64, c_i32, c_p], 1),
+    "pse_rotary_append": ([BlockState, KVLayer, RotarySpec, HeadView, HeadView, HeadView, HeadView, HeadView, c_p, c_p,
+                           c_p, c_i64, c_p], 1),
+    "pse_prompt_plan": ([c_p, c_i32, c_i32, c_i32, c_i32, c_p, c_i64, c_p], 0),
+    "pse_prompt_attention": ([HeadView, HeadView, HeadView, HeadView, c_i64, c_i32, c_i32, c_f32, c_p, c_i32, c_i64,
+                              c_p, c_p], 1),
+    "pse_tree_masks": ([c_p, c_p, c_i32, c_i32, c_i32, c_p, c_p, c_p], 1),
+    "pse_token_tree_attention": ([BlockState, KVLayer, HeadView, HeadView, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_p,
+                                  c_i32, c_f32, c_p, c_sz, c_p], 1),
     "pse_scatter_rows": ([c_p, c_i64, c_p, c_i32, c_i32, c_p, c_i64, c_i32, c_p], 1),
     "pse_attention_force_generic": ([c_i32], 0),
     "pse_accept_select": ([c_i32], 0),
@@ -94,6 +111,7 @@ _PROTOS = {
     "pse_step_finish": ([c_p, c_p, c_p, c_i32, c_p, c_i32, c_p, c_i32, c_p, c_i32, c_p, c_p, c_p, c_p, c_p], 1),
 }
 _SIZE_PROTOS = {
+    "pse_token_tree_workspace": [c_i32],
     "pse_paged_attention_workspace": [c_i32, c_i32, c_i32, c_i32, c_i32, c_i32],
 }
 

@@ -1,0 +1,130 @@
+"""Attention of drafted token trees of any shape over the paged cache.
+
+``pse.tree`` drives trees of equal branches through one kernel rule; here each
+request brings its own tree: any parents, any number of nodes (none included),
+packed over the requests.  Node j of a request stands in the cache at position
+context + j, whatever its depth; its rotary position is context + depth.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native as N
+from .rotary import check_heads, check_index, head_view
+
+MAX_NODES = 4096  # nodes of one request's tree
+
+
+class TokenTrees:
+    """A batch of trees: ``masks`` int64 [nodes, words] (bit m of a node's
+    words: it attends to node m of its own tree), ``counts`` the requests' node
+    counts (host integers)."""
+
+    def __init__(self, masks: torch.Tensor, counts, depths: torch.Tensor | None = None,
+                 offsets: torch.Tensor | None = None) -> None:
+        N.load()
+        self.counts = [int(n) for n in counts]
+        if any(n < 0 for n in self.counts):
+            raise ValueError("a tree's node count is negative")
+        self.nodes, self.max_nodes = sum(self.counts), max(self.counts, default=0)
+        if self.max_nodes > MAX_NODES:
+            raise ValueError(f"a tree of {self.max_nodes} nodes (at most {MAX_NODES})")
+        if not torch.is_tensor(masks) or masks.dim() != 2 or masks.dtype != torch.int64 or not masks.is_cuda or \
+                not masks.is_contiguous() or masks.shape[0] != self.nodes or masks.shape[1] < 1:
+            raise ValueError(f"masks must be a contiguous int64 [{self.nodes}, words] tensor on a GPU")
+        self.words = masks.shape[1]
+        if self.max_nodes > 64 * self.words:
+            raise ValueError(f"{self.words} mask words for a tree of {self.max_nodes} nodes")
+        self.masks, self.depths, self.device = masks, depths, masks.device
+        self.offsets = _offsets(self.counts, self.device) if offsets is None else offsets
+
+    @classmethod
+    def from_parents(cls, parents: torch.Tensor, counts) -> "TokenTrees":
+        """The trees of packed ``parents`` (see ``tree_masks``); ``depths`` is set."""
+        return tree_masks(parents, counts)
+
+
+def _offsets(counts, device) -> torch.Tensor:
+    out = [0]
+    for n in counts:
+        out.append(out[-1] + n)
+    return torch.tensor(out, dtype=torch.int32).to(device, non_blocking=True)
+
+
+def tree_masks(parents: torch.Tensor, counts) -> TokenTrees:
+    """Ancestor masks of packed trees.  ``parents`` int32 [nodes] on the
+    device: a node's parent within its tree (a lower index) or -1 for a child
+    of the context.  Each node sees itself and its ancestors; ``depths`` int32
+    counts the edges above it (0 for a child of the context)."""
+    counts = [int(n) for n in counts]
+    if any(n < 0 for n in counts):
+        raise ValueError("a tree's node count is negative")
+    n = sum(counts)
+    if not torch.is_tensor(parents) or not parents.is_cuda:
+        raise ValueError("parents must be on a GPU")
+    check_index("parents", parents, n, parents.device)
+    words = max(1, (max(counts, default=0) + 63) // 64)
+    offsets = _offsets(counts, parents.device)
+    masks = torch.empty(n, words, dtype=torch.int64, device=parents.device)
+    depths = torch.empty(n, dtype=torch.int32, device=parents.device)
+    trees = TokenTrees(masks, counts, depths, offsets)
+    N.call("pse_tree_masks", parents.data_ptr(), offsets.data_ptr(), len(counts), n, words, masks.data_ptr(),
+           depths.data_ptr(), N.stream_ptr())
+    return trees
+
+
+_workspaces: dict = {}
+
+
+def token_tree_workspace(head_dim: int, device) -> torch.Tensor:
+    """A workspace for ``token_tree_attention`` (its head zeroed).  Calls that
+    may overlap on the GPU need one each."""
+    return torch.zeros(N.size_call("pse_token_tree_workspace", head_dim), dtype=torch.uint8, device=device)
+
+
+def _workspace(head_dim: int, device) -> torch.Tensor:
+    """The current stream's own workspace.  A call under capture gets one of
+    its graph instead, so a replay never shares it with other work."""
+    if torch.cuda.is_current_stream_capturing():
+        return token_tree_workspace(head_dim, device)
+    key = (device, N.stream_ptr())
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < N.size_call("pse_token_tree_workspace", head_dim):
+        ws = _workspaces[key] = token_tree_workspace(head_dim, device)
+    return ws
+
+
+def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor, context: torch.Tensor,
+                         trees: TokenTrees, *, scale: float | None = None, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of every tree node to its request's ``context`` (int32 [rows]
+    tokens in the cache) and to the nodes its mask names.  q [nodes, q_heads,
+    head_dim] in the cache's dtype, any token and head strides; ``slots`` int32
+    [rows] (``cache.slots_tensor``).  The nodes' K/V must be in the cache, node
+    j at position context + j.  ``scale`` defaults to 1 / sqrt(head_dim).
+    Returns [nodes, q_heads, head_dim]; a node that sees nothing gives zeros."""
+    hd = cache.head_dim
+    check_heads("q", q, hd)
+    if q.dtype != cache.dtype or q.device != cache.device or trees.device != q.device:
+        raise ValueError("q, the cache and the trees must match in dtype and device")
+    if q.shape[0] != trees.nodes:
+        raise ValueError(f"{q.shape[0]} queries, but the trees hold {trees.nodes} nodes")
+    if q.shape[1] == 0 or q.shape[1] % cache.n_heads or q.shape[1] // cache.n_heads > 64 or hd > 256:
+        raise ValueError(f"{q.shape[1]} query heads over {cache.n_heads} K/V heads of {hd}")
+    if not 0 <= layer < cache.n_layers:
+        raise ValueError(f"layer {layer} of a cache with {cache.n_layers}")
+    rows = len(trees.counts)
+    check_index("slots", slots, rows, q.device)
+    check_index("context", context, rows, q.device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    check_heads("out", out, hd, q, q.shape[1])
+    if workspace is None:
+        workspace = _workspace(hd, q.device)
+    N.call("pse_token_tree_attention", cache.state, cache.layer(layer), head_view(q), head_view(out),
+           slots.data_ptr(), context.data_ptr(), trees.offsets.data_ptr(), rows, trees.nodes, trees.max_nodes,
+           trees.masks.data_ptr(), trees.words, 1.0 / math.sqrt(hd) if scale is None else float(scale),
+           workspace.data_ptr(), workspace.numel(), N.stream_ptr())
+    return out
