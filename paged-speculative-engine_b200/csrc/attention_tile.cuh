@@ -1,0 +1,107 @@
+// The softmax of one 128 x 128 score tile, shared by the prompt and tree
+// kernels: scores come from tensor memory, weights go back there as bf16.
+#pragma once
+
+#include "tcgen05.cuh"
+
+namespace pse {
+namespace tile {
+
+using namespace t5;
+
+constexpr int kKeys = 128;
+
+// A query row's running statistics, in units of log2: weights are taken
+// against `m`, a maximum of the row's scores so far that is raised only when
+// the true maximum has passed it by more than 8.  The weights stay below 2^8,
+// the output then needs no rescaling in most tiles, and the quotient O / l is
+// the same whatever reference both were taken against.
+struct RowState {
+  float m, l;
+  __device__ void reset() {
+    m = -INFINITY;
+    l = 0.f;
+  }
+};
+
+// One tile of one row (this thread's TMEM lane).  s_col: the 128 score columns,
+// whose first 64 columns receive the weights, two bf16 to a column.  o_col: the
+// row's HD output columns, rescaled here when `first` is false and the
+// reference maximum moved.  masked (warp-uniform): only keys whose bit is set
+// in vis[0..3] take part.  half_done[h] is arrived on (once per warp) when the
+// weights of keys 64 h .. 64 h + 63 stand in tensor memory.
+//
+// The weights are rounded to bf16 for the tensor cores (the sum l adds them
+// unrounded in fp32): 2^-8 of a weight at most, as much as the bf16 result's
+// own rounding.
+template <int HD>
+__device__ __forceinline__ void softmax_tile(uint32_t lane_base, uint32_t s_col, uint32_t o_col, float sl2, bool first,
+                                             bool masked, const uint32_t* vis, RowState& row, uint64_t* half0,
+                                             uint64_t* half1) {
+  uint32_t u[kKeys];
+  float* s = reinterpret_cast<float*>(u);
+#pragma unroll
+  for (int c = 0; c < kKeys / 32; ++c) tmem_ld32(lane_base + s_col + 32 * c, u + 32 * c);
+  tmem_wait_ld();
+  if (masked) {
+#pragma unroll
+    for (int c = 0; c < kKeys; ++c) s[c] = (vis[c >> 5] >> (c & 31)) & 1u ? s[c] : -INFINITY;
+  }
+  float m4[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) m4[x] = fmaxf(s[x], s[x + 4]);
+#pragma unroll
+  for (int c = 8; c < kKeys; c += 8) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) m4[x] = fmaxf(fmaxf(m4[x], s[c + x]), s[c + 4 + x]);
+  }
+  const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
+  float corr = 1.f;
+  if (mx > row.m + 8.f) {
+    corr = ex2(row.m - mx);  // 0 from -inf
+    row.m = mx;
+  }
+  row.l *= corr;
+  if (!first && __any_sync(0xffffffffu, corr != 1.f)) {
+    // every product issued before these scores has retired (their commit
+    // covers it), so the output can be rescaled in place
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld32(lane_base + o_col + 32 * c, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+      tmem_st32(lane_base + o_col + 32 * c, o);
+    }
+  }
+  const float neg = row.m == -INFINITY ? 0.f : -row.m;
+  const uint64_t sc2 = pack2(sl2, sl2), neg2 = pack2(neg, neg);
+  uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t p[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int c = 64 * h + 2 * i;
+      float lo, hi;
+      unpack2(fma2(pack2(s[c], s[c + 1]), sc2, neg2), lo, hi);
+      lo = ex2(lo);
+      hi = ex2(hi);
+      sum[i & 1] = add2(sum[i & 1], pack2(lo, hi));
+      p[i] = pack_bf16(lo, hi);
+    }
+    tmem_st32(lane_base + s_col + 32 * h, p);
+    tmem_wait_st();
+    fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(h == 0 ? half0 : half1);
+  }
+  float a, b, c, d;
+  unpack2(sum[0], a, b);
+  unpack2(sum[1], c, d);
+  row.l += (a + b) + (c + d);
+}
+
+}  // namespace tile
+}  // namespace pse

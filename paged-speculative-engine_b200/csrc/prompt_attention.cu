@@ -13,6 +13,7 @@
 #include <queue>
 #include <vector>
 
+#include "attention_tile.cuh"
 #include "simt_attention.cuh"
 
 namespace pse {
@@ -120,6 +121,431 @@ int simt_attention(const Args& a, cudaStream_t s) {
   if (a.hd <= 64) return launch_simt<T, 1>(a, s);
   if (a.hd <= 128) return launch_simt<T, 2>(a, s);
   return launch_simt<T, 4>(a, s);
+}
+
+// ---------------------------------------------------------------- tensor cores
+// bf16, head_dim 64 or 128.  A CTA per multiprocessor works through its list of
+// items.  A query tile is 128 rows, (token, group head) token-major; an item's
+// two tiles are two streams that share every 128-key K/V tile:
+//   warps 0-3, 4-7  the softmax of stream 0 and 1, a thread per row
+//                   (attention_tile.cuh), and the item's output
+//   warp 8          TMA: Q tiles, and K and V tiles through a ring of slots
+//   warp 9          one thread issues the products: S = Q K^T into tensor
+//                   memory, O += P V with P there (over S's columns), V MN-major
+//   warp 10         looks through V tiles that some row must not see in whole
+// While a stream's softmax runs, the tensor cores work on the other stream.
+//
+// A hidden key has weight zero, but 0 x inf is NaN in a product, and a tile at
+// the causal edge or the prompt's end holds V rows of later tokens or of the
+// next prompt.  Warp 10 zeroes the infinities and NaN of such a tile before the
+// product sees it and marks the tile; at the item's end a row adds the marked
+// tiles' non-finite values of the keys it does see.
+using namespace t5;
+
+constexpr int kTcThreads = 384;
+constexpr int kHalfBytes = 128 * 128;  // 64 columns of a 128-row tile
+constexpr int kGuards = 8;             // barriers of tiles on their way through warp 10
+constexpr uint32_t kColS = 0, kColO = 256;
+
+template <int HD>
+__host__ __device__ constexpr int n_slots() { return HD == 128 ? 5 : 8; }
+
+template <int HD>
+constexpr size_t tc_smem_bytes() {
+  return 1024 + (size_t)2 * 128 * HD * 2 + (size_t)n_slots<HD>() * 128 * HD * 2 + 512;
+}
+
+struct TcItem {
+  int tok0, len, w0, hk;
+  int n[2], n_max;
+  int guard0;  // first tile that its first row does not see in whole
+};
+
+__device__ __forceinline__ TcItem decode(const Args& a, int e, int tpt) {
+  const int4 x = __ldg(reinterpret_cast<const int4*>(a.plan + plan_items_at(a.n_cta)) + e);
+  TcItem it;
+  it.tok0 = x.x;
+  it.len = x.y;
+  it.w0 = x.z;
+  it.hk = x.w;
+  const bool ok = it.tok0 >= 0 && it.len >= 0 && it.w0 >= 0 && (int64_t)it.tok0 + it.len <= a.tokens && it.hk >= 0 &&
+                  it.hk < a.kv_heads;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int first = it.w0 + s * tpt;
+    it.n[s] = ok && first < it.len ? (min(first + tpt, it.len) + 127) >> 7 : 0;
+  }
+  it.n_max = max(it.n[0], it.n[1]);
+  it.guard0 = (it.w0 + 1) >> 7;
+  return it;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    prompt_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                     const __grid_constant__ CUtensorMap tmv, const Args a) {
+  constexpr int NS = n_slots<HD>();
+  constexpr int kTileBytes = 128 * HD * 2, kHalves = HD / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;                     // [2 streams][128 x HD]
+  uint8_t* ring = q_s + 2 * kTileBytes;    // [NS][128 x HD]: K and V tiles in turn
+  uint64_t* slot_full = reinterpret_cast<uint64_t*>(ring + NS * kTileBytes);
+  uint64_t* slot_empty = slot_full + NS;
+  uint64_t* guard_full = slot_empty + NS;  // [kGuards] a guarded V tile landed
+  uint64_t* q_full = guard_full + kGuards;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;          // [2] a stream's scores stand in tensor memory
+  uint64_t* p_half = s_full + 2;           // [2][2] half of a stream's weights stand there
+  uint64_t* o_full = p_half + 4;           // [2] a stream's last product of the item retired
+  uint64_t* o_empty = o_full + 2;          // [2] its output has been read
+  uint64_t* final_bar = o_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  int* poison = abort_flag + 1;            // [kGuards] items' marked tiles, bit j: tile guard0 + j
+  int* last_bar = poison + kGuards;        // [NS + 1] per slot (and Q): barrier and parity of its last copy
+  volatile int* vabort = abort_flag;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&slot_full[i], 1);
+      mbar_init(&slot_empty[i], 1);
+    }
+    for (int i = 0; i < kGuards; ++i) mbar_init(&guard_full[i], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_half[2 * s], 4);
+      mbar_init(&p_half[2 * s + 1], 4);
+      mbar_init(&o_full[s], 1);
+      mbar_init(&o_empty[s], 4);
+    }
+    mbar_init(final_bar, 1);
+    *abort_flag = 0;
+    for (int i = 0; i <= NS; ++i) last_bar[i] = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  const int tpt = tile_tokens(a.group);
+  const int e0 = __ldg(a.plan + blockIdx.x), e1 = min(__ldg(a.plan + blockIdx.x + 1), a.n_items);
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8) {
+      // -------------------------------------------------------------- copies
+      if (lane == 0) {
+        int c = 0, g = 0, nq = 0;
+        bool run = true;
+        auto load = [&](const CUtensorMap* map, int hk, int tok, bool guarded) -> bool {
+          const int s = c % NS;
+          if (!mbar_wait(&slot_empty[s], ((c / NS) & 1) ^ 1, vabort)) return false;
+          uint64_t* bar = guarded ? &guard_full[g % kGuards] : &slot_full[s];
+          last_bar[s] = guarded ? (NS + g % kGuards) * 2 + ((g / kGuards) & 1) : s * 2 + ((c / NS) & 1);
+          mbar_expect_tx(bar, kTileBytes);
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            tma_load_3d(ring + s * kTileBytes + h * kHalfBytes, map, h * 64, hk, tok, bar);
+          ++c;
+          if (guarded) ++g;
+          return true;
+        };
+        for (int e = e0; run && e < e1; ++e) {
+          const TcItem it = decode(a, e, tpt);
+          if (it.n_max == 0) continue;
+          if (!mbar_wait(q_empty, (nq & 1) ^ 1, vabort)) break;
+          const int streams = it.n[1] > 0 ? 2 : 1;
+          last_bar[NS] = nq & 1;
+          mbar_expect_tx(q_full, streams * kHalves * tpt * a.group * 128);
+          for (int s = 0; s < streams; ++s)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_3d(q_s + s * kTileBytes + h * kHalfBytes, &tmq, h * 64, it.hk * a.group,
+                          it.tok0 + it.w0 + s * tpt, q_full);
+          ++nq;
+          for (int j = 0; run && j < it.n_max; ++j)
+            run = load(&tmk, it.hk, it.tok0 + j * 128, false) && load(&tmv, it.hk, it.tok0 + j * 128, j >= it.guard0);
+        }
+      }
+    } else if (warp == 9) {
+      // -------------------------------------------------------------- products
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = instr_desc(128, 0), idesc_o = instr_desc(HD, 1);
+        constexpr uint32_t kVAtoms = HD == 128 ? (uint32_t)kHalfBytes : 1024u;
+        int c = 0;             // slots used by earlier tiles: K of tile j at c + 2 j, V at c + 2 j + 1
+        int np[2] = {0, 0};    // weights consumed per stream
+        int no[2] = {0, 0};    // items finished per stream
+        int nq = 0;
+        bool run = true;
+        auto slot_wait = [&](int x) { return mbar_wait(&slot_full[x % NS], (x / NS) & 1, vabort); };
+        auto scores = [&](int s, int x) {
+          const uint32_t qa = su32(q_s + s * kTileBytes), kb = su32(ring + (x % NS) * kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+            mma_ss(tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
+          }
+          mma_commit(&s_full[s]);
+        };
+        for (int e = e0; run && e < e1; ++e) {
+          const TcItem it = decode(a, e, tpt);
+          if (it.n_max == 0) continue;
+          if (!mbar_wait(q_full, nq & 1, vabort) || !slot_wait(c)) break;
+          ++nq;
+          fence_after();
+          for (int s = 0; s < 2; ++s)
+            if (it.n[s] > 0) scores(s, c);
+          mma_commit(&slot_empty[c % NS]);
+          if (it.n_max == 1) mma_commit(q_empty);
+          for (int j = 0; run && j < it.n_max; ++j) {
+            const int kx = c + 2 * (j + 1), vx = c + 2 * j + 1;
+            bool v_here = false, k_here = false;
+            for (int s = 0; run && s < 2; ++s) {
+              if (j >= it.n[s]) continue;
+              if (!v_here) run = slot_wait(vx);
+              v_here = true;
+              if (run && j == 0 && no[s] > 0) run = mbar_wait(&o_empty[s], (no[s] - 1) & 1, vabort);
+              const uint32_t vb = su32(ring + (vx % NS) * kTileBytes);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (run) run = mbar_wait(&p_half[2 * s + h], np[s] & 1, vabort);
+                if (!run) break;
+                fence_after();
+#pragma unroll
+                for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                  mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
+                         idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+              }
+              if (!run) break;
+              ++np[s];
+              if (j + 1 == it.n[s]) {
+                mma_commit(&o_full[s]);
+                ++no[s];
+              } else {
+                if (!k_here) run = slot_wait(kx);
+                k_here = true;
+                if (!run) break;
+                fence_after();
+                scores(s, kx);
+              }
+            }
+            if (!run) break;
+            mma_commit(&slot_empty[vx % NS]);
+            if (k_here) {
+              mma_commit(&slot_empty[kx % NS]);
+              if (j + 2 == it.n_max) mma_commit(q_empty);
+            }
+          }
+          c += 2 * it.n_max;
+        }
+        mma_commit(final_bar);
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      // -------------------------------------------------------------- guard
+      int c = 0, g = 0, items = 0;
+      bool run = true;
+      for (int e = e0; run && e < e1; ++e) {
+        const TcItem it = decode(a, e, tpt);
+        if (it.n_max == 0) continue;
+        int marks = 0;
+        for (int j = it.guard0; j < it.n_max; ++j, ++g) {
+          if (!mbar_wait_warp(&guard_full[g % kGuards], (g / kGuards) & 1, vabort)) {
+            run = false;
+            break;
+          }
+          const int s = (c + 2 * j + 1) % NS;
+          uint4* v = reinterpret_cast<uint4*>(ring + s * kTileBytes);
+          // 0 x value summed over a chunk is NaN if any value is not finite
+          bool bad = false;
+          for (int i = lane; i < kTileBytes / 16; i += 32 * 8) {
+            __nv_bfloat162 z = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const uint4 w = v[i + 32 * x];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const uint32_t b = y == 0 ? w.x : y == 1 ? w.y : y == 2 ? w.z : w.w;
+                z = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&b), __floats2bfloat162_rn(0.f, 0.f), z);
+              }
+            }
+            bad |= !(__low2float(z) == 0.f && __high2float(z) == 0.f);
+          }
+          if (__any_sync(0xffffffffu, bad)) {
+            marks |= 1 << (j - it.guard0);
+            uint32_t* w = reinterpret_cast<uint32_t*>(v);
+            for (int i = lane; i < kTileBytes / 4; i += 32) {
+              uint32_t x = w[i];
+              if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+              if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
+              w[i] = x;
+            }
+            fence_proxy();
+          }
+          __syncwarp();
+          if (lane == 0) {
+            poison[items % kGuards] = marks;
+            mbar_arrive(&slot_full[s]);
+          }
+        }
+        c += 2 * it.n_max;
+        ++items;
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int s = warp >> 2, r = tid & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const int rt = r / a.group, rg = r - rt * a.group;
+    int nt = 0, items = 0, no = 0;  // tiles, items and outputs of this stream
+    bool run = true;
+    for (int e = e0; run && e < e1; ++e) {
+      const TcItem it = decode(a, e, tpt);
+      if (it.n_max == 0) continue;
+      const int item = items++;
+      if (it.n[s] == 0) continue;
+      const int tok = it.w0 + s * tpt + rt;  // this row's token within its prompt
+      const bool valid = rt < tpt && tok < it.len;
+      const int lim = valid ? tok + 1 : 0x7fffffff;  // keys [0, lim) are visible
+      const bool any_valid = __any_sync(0xffffffffu, valid);
+      tile::RowState row;
+      row.reset();
+      for (int j = 0; j < it.n[s]; ++j, ++nt) {
+        if (!mbar_wait_warp(&s_full[s], nt & 1, vabort)) {
+          run = false;
+          break;
+        }
+        fence_after();
+        if (!any_valid) {
+          // no row of this warp is anyone's: its weights may be anything
+          if (lane == 0) {
+            mbar_arrive(&p_half[2 * s]);
+            mbar_arrive(&p_half[2 * s + 1]);
+          }
+          continue;
+        }
+        const int left = lim - j * 128;
+        const bool masked = __any_sync(0xffffffffu, left < 128);
+        uint32_t vis[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int n = left - 32 * x;
+          vis[x] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+        }
+        tile::softmax_tile<HD>(lane_base, kColS + s * 128, kColO + s * 128, a.scale_log2, j == 0, masked, vis, row,
+                               &p_half[2 * s], &p_half[2 * s + 1]);
+      }
+      if (!run || !mbar_wait_warp(&o_full[s], no & 1, vabort)) break;
+      ++no;
+      fence_after();
+      const int marks = it.guard0 < it.n_max ? poison[item % kGuards] : 0;
+      // a row whose weights are all zero (every score -inf) gives zero
+      const float inv = row.l == 0.f ? 0.f : 1.f / row.l;
+      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + (int64_t)(it.tok0 + tok) * a.o_tok +
+                           (int64_t)(it.hk * a.group + rg) * a.o_head;
+#pragma unroll
+      for (int h = 0; h < HD / 32; ++h) {
+        uint32_t u[32];
+        float* o = reinterpret_cast<float*>(u);
+        tmem_ld32(lane_base + kColO + s * 128 + 32 * h, u);
+        tmem_wait_ld();
+        if (h == HD / 32 - 1) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[s]);
+        }
+        if (marks && valid) {
+          const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(a.v) + it.hk * a.v_head + 32 * h;
+#pragma unroll 1
+          for (int key = it.guard0 * 128; key < lim; ++key) {
+            if (!(marks >> ((key >> 7) - it.guard0) & 1)) continue;
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const float y = __bfloat162float(v[(int64_t)(it.tok0 + key) * a.v_tok + x]);
+              if (!isfinite(y)) o[x] += y;
+            }
+          }
+        }
+        if (valid) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            uint4 w;
+            w.x = pack_bf16(o[x] * inv, o[x + 1] * inv);
+            w.y = pack_bf16(o[x + 2] * inv, o[x + 3] * inv);
+            w.z = pack_bf16(o[x + 4] * inv, o[x + 5] * inv);
+            w.w = pack_bf16(o[x + 6] * inv, o[x + 7] * inv);
+            *reinterpret_cast<uint4*>(dst + 32 * h + x) = w;
+          }
+        }
+      }
+    }
+  }
+
+  __syncthreads();
+  if (*vabort) {
+    if (tid == 0 && a.status) atomicOr(a.status, PSE_STATUS_TIMEOUT);
+    if (tid == 0) {
+      // copies still on their way land before the shared memory goes
+      for (int i = 0; i < NS; ++i)
+        if (last_bar[i] >= 0) {
+          const int b = last_bar[i] >> 1;
+          mbar_drain(b < NS ? &slot_full[b] : &guard_full[b - NS], last_bar[i] & 1);
+        }
+      if (last_bar[NS] >= 0) mbar_drain(q_full, last_bar[NS]);
+    }
+  }
+  if (warp == 9) {
+    if (lane == 0) mbar_drain(final_bar, 0);
+    __syncwarp();
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+Map3Cache g_maps;
+
+bool tc_view(const char* p, int64_t tok, int64_t head, int heads, int hd) {
+  if (heads == 1) head = hd;  // the stride of an axis of one is not used
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= hd && head >= hd &&
+         tok < (1ll << 38) && head < (1ll << 38);
+}
+
+bool tc_eligible(const Args& a) {
+  return (a.hd == 64 || a.hd == 128) && a.group <= 128 && a.scale_log2 > 0.f &&
+         tc_view(a.q, a.q_tok, a.q_head, a.q_heads, a.hd) && tc_view(a.k, a.k_tok, a.k_head, a.kv_heads, a.hd) &&
+         tc_view(a.v, a.v_tok, a.v_head, a.kv_heads, a.hd) && tc_view(a.out, a.o_tok, a.o_head, a.q_heads, a.hd);
+}
+
+template <int HD>
+int launch_tc(const Args& a, cudaStream_t s) {
+  auto kern = prompt_tc_kernel<HD>;
+  constexpr size_t smem = tc_smem_bytes<HD>();
+  static_assert(smem <= 227 * 1024, "shared memory");
+  static const cudaError_t opt = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (opt != cudaSuccess) return (int)opt;
+  auto key = [&](const char* p, int64_t tok, int64_t head, int heads, uint32_t b1, uint32_t b2) {
+    return Map3Key{reinterpret_cast<uint64_t>(p), (uint64_t)HD, (uint64_t)heads, (uint64_t)a.tokens,
+                   (uint64_t)(heads == 1 ? HD : head) * 2, (uint64_t)tok * 2, b1, b2};
+  };
+  CUtensorMap mq, mk, mv;
+  int rc = g_maps.get(key(a.q, a.q_tok, a.q_head, a.q_heads, a.group, tile_tokens(a.group)), &mq);
+  if (rc == 0) rc = g_maps.get(key(a.k, a.k_tok, a.k_head, a.kv_heads, 1, 128), &mk);
+  if (rc == 0) rc = g_maps.get(key(a.v, a.v_tok, a.v_head, a.kv_heads, 1, 128), &mv);
+  if (rc) return rc;
+  // with fewer items than CTAs the plan gives them to the first ones
+  const int grid = a.n_items < a.n_cta ? a.n_items : a.n_cta;
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kTcThreads), smem, s, mq, mk, mv, a);
+  return e == cudaSuccess ? PSE_OK : (int)e;
 }
 
 // ---------------------------------------------------------------- planning
@@ -230,6 +656,9 @@ extern "C" int pse_prompt_attention(pse_head_view q, pse_head_view k, pse_head_v
   a.n_cta = n_cta;
   a.n_items = (int)n_items;
   a.status = status;
+  if (dtype == PSE_BF16 && prompt::tc_eligible(a))
+    return head_dim == 64 ? prompt::launch_tc<64>(a, (cudaStream_t)stream)
+                          : prompt::launch_tc<128>(a, (cudaStream_t)stream);
   return dtype == PSE_BF16 ? prompt::simt_attention<__nv_bfloat16>(a, (cudaStream_t)stream)
                            : prompt::simt_attention<float>(a, (cudaStream_t)stream);
 }
