@@ -429,7 +429,7 @@ int pse_prompt_plan(const int32_t *lens, int32_t n, int32_t q_heads, int32_t kv_
  * token i of a prompt attends to tokens 0..i of that prompt, query head h to K/V
  * head h / (q.heads / k.heads); head_dim <= 256.  A row whose weights sum to
  * zero gives zero.  bf16 with head_dim 64 or 128, at most 128 heads a group and
- * 16-byte aligned rows runs on the tensor cores, the rest in fp32 on the CUDA
+ * 16-byte aligned q, k, v rows runs on the tensor cores, the rest in fp32 on the CUDA
  * cores.  Items that lie outside the tensors are skipped.  `status` (nullable)
  * receives PSE_STATUS_TIMEOUT if a bounded in-kernel wait expires.  `plan` is
  * the device copy of pse_prompt_plan's list. */
@@ -458,7 +458,7 @@ int pse_tree_masks(const int32_t *parents, const int32_t *node_off, int32_t rows
  * table cannot hold.  max_nodes bounds the rows' node counts (it picks the
  * kernel's shape; max_nodes <= 64 words).  ctx, slots and node_off are read on
  * the device only, so the call can be captured and replayed with other values.
- * workspace: pse_token_tree_workspace() bytes, 16-byte aligned, the first 2048
+ * workspace: pse_token_tree_workspace() bytes, 16-byte aligned, the first 8192
  * of them zero before the first call and zero again after every call; calls
  * that share one must not overlap on the GPU. */
 int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,

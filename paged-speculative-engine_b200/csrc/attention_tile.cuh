@@ -103,5 +103,64 @@ __device__ __forceinline__ void softmax_tile(uint32_t lane_base, uint32_t s_col,
   row.l += (a + b) + (c + d);
 }
 
+// 32 columns of an output row, scaled and rounded; vec: the row is 16-byte aligned.
+__device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const float* o, float inv, bool vec) {
+#pragma unroll
+  for (int x = 0; x < 32; x += 8) {
+    uint4 w;
+    w.x = pack_bf16(o[x] * inv, o[x + 1] * inv);
+    w.y = pack_bf16(o[x + 2] * inv, o[x + 3] * inv);
+    w.z = pack_bf16(o[x + 4] * inv, o[x + 5] * inv);
+    w.w = pack_bf16(o[x + 6] * inv, o[x + 7] * inv);
+    if (vec) {
+      *reinterpret_cast<uint4*>(dst + x) = w;
+    } else {
+      unsigned short* d = reinterpret_cast<unsigned short*>(dst + x);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t v = y == 0 ? w.x : y == 1 ? w.y : y == 2 ? w.z : w.w;
+        d[2 * y] = (unsigned short)v;
+        d[2 * y + 1] = (unsigned short)(v >> 16);
+      }
+    }
+  }
+}
+
+// A whole warp: sets the infinities and NaN among n vectors of 8 bf16 (n a
+// multiple of 256) in shared memory to zero, visible to later products; returns
+// whether there were any.
+__device__ __forceinline__ bool clear_nonfinite(uint4* v, int n) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+  bool bad = false;
+  for (int i = lane; i < n; i += 256) {
+    // 0 x value, summed: NaN if any value is not finite, else a zero
+    __nv_bfloat162 z = zero;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const uint4 w = v[i + 32 * x];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t b = y == 0 ? w.x : y == 1 ? w.y : y == 2 ? w.z : w.w;
+        z = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&b), zero, z);
+      }
+    }
+    bad |= !(__low2float(z) == 0.f && __high2float(z) == 0.f);
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  if (bad) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(v);
+    for (int i = lane; i < 4 * n; i += 32) {
+      uint32_t x = w[i];
+      if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+      if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
+      w[i] = x;
+    }
+    fence_proxy();
+  }
+  __syncwarp();
+  return bad;
+}
+
 }  // namespace tile
 }  // namespace pse

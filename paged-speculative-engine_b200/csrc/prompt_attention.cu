@@ -29,6 +29,7 @@ struct Args {
   const int32_t* plan;  // [n_cta + 1] first items, padding, then int4 {first token, length, first query token, K/V head}
   int n_cta, n_items;
   int32_t* status;
+  bool out_vec;  // output rows are 16-byte aligned
 };
 
 // Tokens of one query tile: at most 128 rows of (token, group head).
@@ -129,10 +130,11 @@ int simt_attention(const Args& a, cudaStream_t s) {
 // two tiles are two streams that share every 128-key K/V tile:
 //   warps 0-3, 4-7  the softmax of stream 0 and 1, a thread per row
 //                   (attention_tile.cuh), and the item's output
-//   warp 8          TMA: Q tiles, and K and V tiles through a ring of slots
+//   warp 8          TMA: K and V tiles through a ring of slots
 //   warp 9          one thread issues the products: S = Q K^T into tensor
 //                   memory, O += P V with P there (over S's columns), V MN-major
 //   warp 10         looks through V tiles that some row must not see in whole
+//   warp 11         TMA: Q tiles, so that the ring runs on into the next item
 // While a stream's softmax runs, the tensor cores work on the other stream.
 //
 // A hidden key has weight zero, but 0 x inf is NaN in a product, and a tile at
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 8) {
       // -------------------------------------------------------------- copies
       if (lane == 0) {
-        int c = 0, g = 0, nq = 0;
+        int c = 0, g = 0;
         bool run = true;
         auto load = [&](const CUtensorMap* map, int hk, int tok, bool guarded) -> bool {
           const int s = c % NS;
@@ -262,6 +264,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int e = e0; run && e < e1; ++e) {
           const TcItem it = decode(a, e, tpt);
           if (it.n_max == 0) continue;
+          for (int j = 0; run && j < it.n_max; ++j)
+            run = load(&tmk, it.hk, it.tok0 + j * 128, false) && load(&tmv, it.hk, it.tok0 + j * 128, j >= it.guard0);
+        }
+      }
+    } else if (warp == 11) {
+      // -------------------------------------------------------------- queries
+      if (lane == 0) {
+        int nq = 0;
+        for (int e = e0; e < e1; ++e) {
+          const TcItem it = decode(a, e, tpt);
+          if (it.n_max == 0) continue;
           if (!mbar_wait(q_empty, (nq & 1) ^ 1, vabort)) break;
           const int streams = it.n[1] > 0 ? 2 : 1;
           last_bar[NS] = nq & 1;
@@ -272,8 +285,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tma_load_3d(q_s + s * kTileBytes + h * kHalfBytes, &tmq, h * 64, it.hk * a.group,
                           it.tok0 + it.w0 + s * tpt, q_full);
           ++nq;
-          for (int j = 0; run && j < it.n_max; ++j)
-            run = load(&tmk, it.hk, it.tok0 + j * 128, false) && load(&tmv, it.hk, it.tok0 + j * 128, j >= it.guard0);
         }
       }
     } else if (warp == 9) {
@@ -364,34 +375,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             break;
           }
           const int s = (c + 2 * j + 1) % NS;
-          uint4* v = reinterpret_cast<uint4*>(ring + s * kTileBytes);
-          // 0 x value summed over a chunk is NaN if any value is not finite
-          bool bad = false;
-          for (int i = lane; i < kTileBytes / 16; i += 32 * 8) {
-            __nv_bfloat162 z = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const uint4 w = v[i + 32 * x];
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const uint32_t b = y == 0 ? w.x : y == 1 ? w.y : y == 2 ? w.z : w.w;
-                z = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&b), __floats2bfloat162_rn(0.f, 0.f), z);
-              }
-            }
-            bad |= !(__low2float(z) == 0.f && __high2float(z) == 0.f);
-          }
-          if (__any_sync(0xffffffffu, bad)) {
+          if (tile::clear_nonfinite(reinterpret_cast<uint4*>(ring + s * kTileBytes), kTileBytes / 16))
             marks |= 1 << (j - it.guard0);
-            uint32_t* w = reinterpret_cast<uint32_t*>(v);
-            for (int i = lane; i < kTileBytes / 4; i += 32) {
-              uint32_t x = w[i];
-              if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
-              if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
-              w[i] = x;
-            }
-            fence_proxy();
-          }
-          __syncwarp();
           if (lane == 0) {
             poison[items % kGuards] = marks;
             mbar_arrive(&slot_full[s]);
@@ -477,15 +462,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         if (valid) {
-#pragma unroll
-          for (int x = 0; x < 32; x += 8) {
-            uint4 w;
-            w.x = pack_bf16(o[x] * inv, o[x + 1] * inv);
-            w.y = pack_bf16(o[x + 2] * inv, o[x + 3] * inv);
-            w.z = pack_bf16(o[x + 4] * inv, o[x + 5] * inv);
-            w.w = pack_bf16(o[x + 6] * inv, o[x + 7] * inv);
-            *reinterpret_cast<uint4*>(dst + 32 * h + x) = w;
-          }
+          tile::store_row32(dst + 32 * h, o, inv, a.out_vec);
         }
       }
     }
@@ -523,7 +500,7 @@ bool tc_view(const char* p, int64_t tok, int64_t head, int heads, int hd) {
 bool tc_eligible(const Args& a) {
   return (a.hd == 64 || a.hd == 128) && a.group <= 128 && a.scale_log2 > 0.f &&
          tc_view(a.q, a.q_tok, a.q_head, a.q_heads, a.hd) && tc_view(a.k, a.k_tok, a.k_head, a.kv_heads, a.hd) &&
-         tc_view(a.v, a.v_tok, a.v_head, a.kv_heads, a.hd) && tc_view(a.out, a.o_tok, a.o_head, a.q_heads, a.hd);
+         tc_view(a.v, a.v_tok, a.v_head, a.kv_heads, a.hd);
 }
 
 template <int HD>
@@ -656,6 +633,7 @@ extern "C" int pse_prompt_attention(pse_head_view q, pse_head_view k, pse_head_v
   a.n_cta = n_cta;
   a.n_items = (int)n_items;
   a.status = status;
+  a.out_vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
   if (dtype == PSE_BF16 && prompt::tc_eligible(a))
     return head_dim == 64 ? prompt::launch_tc<64>(a, (cudaStream_t)stream)
                           : prompt::launch_tc<128>(a, (cudaStream_t)stream);

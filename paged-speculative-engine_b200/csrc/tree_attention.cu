@@ -6,14 +6,16 @@
 //
 // The context's K/V is read from HBM once per request, which bounds the call
 // until a K/V head has about 256 query rows (nodes x group).
+#include "attention_tile.cuh"
 #include "simt_attention.cuh"
+#include "tmap_cache.h"
 #include "tree_partition.cuh"
 
 namespace pse {
 namespace tree {
 
 constexpr int kMaxCtas = 2 * kNumSMs;
-constexpr int kCounterBytes = 4 * 512;
+constexpr int kCounterBytes = 8192;  // a counter per CTA, or per softmax warp of one
 
 struct Args {
   Rows rows;
@@ -33,6 +35,7 @@ struct Args {
   int32_t* counters;  // [kMaxCtas], zero between calls
   float* parts;       // [ctas][2][block rows][hd + 2]
   int32_t* status;
+  bool out_vec;  // output rows are 16-byte aligned
 };
 
 // Which of its CTA's two partial results a segment writes: the first segment's
@@ -151,10 +154,8 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
       for (int c = c1; c <= c2; ++c) {
         const float* p = part(a, c, c == c1, BQ) + (int64_t)r * (hd + 2);
         const float f = exp2f(__ldcg(p + hd) - ms);
-        if (f != 0.f) {
-          L += __ldcg(p + hd + 1) * f;
-          x += __ldcg(p + d) * f;
-        }
+        L += __ldcg(p + hd + 1) * f;  // a sum is finite or the NaN of a score
+        if (f != 0.f) x += __ldcg(p + d) * f;
       }
       out_row(r)[d] = from_f32<T>(L == 0.f ? 0.f : x / L);
     }
@@ -188,6 +189,625 @@ int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
   const int rpt = simt_rows(max_nodes * a.rows.group);
   a.block_nodes = 16 * rpt / a.rows.group;
   return rpt == 1 ? simt_nc<T, 1>(a, kMaxCtas, s) : simt_nc<T, 4>(a, kMaxCtas, s);
+}
+
+// ---------------------------------------------------------------- tensor cores
+// bf16 pools, head_dim 64 or 128, pages of 16, 32, 64 or 128 tokens.  One CTA
+// per multiprocessor walks its tiles of the line (tree_partition.cuh).  A query
+// tile is 128 rows, (node, group head) node-major.  Two softmax streams:
+//   NQ = 2 (more than 128 rows per K/V head): two query tiles share every K/V
+//          tile, one per stream;
+//   NQ = 1: both streams hold the same query tile and take the key tiles in
+//          turn, each with an output of its own; at a segment's end the two are
+//          joined, each stream's warps writing half of the columns (warps w and
+//          w + 4 reach the same TMEM lanes, so no output crosses shared memory).
+// Either way one stream's softmax runs beside the other's products.  Warps:
+//   0-3, 4-7  the streams' softmax (attention_tile.cuh), a thread per row
+//   8         K and V pages by TMA into a ring of 128-key slots
+//   9         one thread issues the products
+//   10        clears V tiles that hold nodes (or what stands after them) of
+//             infinities and NaN before the product, as in prompt_attention.cu
+//   11        Q tiles, so that the ring runs on into the next segment
+using namespace t5;
+
+constexpr int kTcThreads = 384;
+constexpr int kHalfBytes = 128 * 128;
+constexpr int kGuards = 8;
+constexpr uint32_t kColS = 0, kColO = 256;
+
+template <int HD, int NQ>
+__host__ __device__ constexpr int n_slots() { return HD == 128 ? 5 : 10; }
+
+template <int HD, int NQ>
+constexpr size_t tc_smem_bytes() {
+  return 1024 + (size_t)(NQ + n_slots<HD, NQ>()) * 128 * HD * 2 + 640 + (NQ == 1 ? 4096 : 0);
+}
+
+// One softmax warp's partial results: 32 rows of HDS columns, then 32 (maximum, sum).
+template <int HDS>
+__device__ __forceinline__ float* warp_part(const Args& a, int cta, bool starts_item, int w) {
+  return a.parts + (((int64_t)cta * 2 + (starts_item ? 1 : 0)) * 8 + w) * 32 * (HDS + 2);
+}
+
+// The last warp to arrive joins the parts of its 32 rows, lanes over the columns.
+template <int HDS, typename F>
+__device__ __forceinline__ void join_parts(const Args& a, int c1, int c2, int w, uint32_t rows, F out_row) {
+  constexpr int kPer = HDS / 32;
+  const int lane = threadIdx.x & 31;
+  while (rows) {
+    const int rr = __ffs(rows) - 1;
+    rows &= rows - 1;
+    float M = -INFINITY;
+    for (int c = c1 + lane; c <= c2; c += 32)
+      M = fmaxf(M, __ldcg(warp_part<HDS>(a, c, c == c1, w) + 32 * HDS + 2 * rr));
+    M = warp_max(M);
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[kPer];
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) acc[x] = 0.f;
+    for (int c0 = c1; c0 <= c2; c0 += 32) {
+      const int n = min(32, c2 + 1 - c0);
+      float f = 0.f, l = 0.f;
+      if (lane < n) {
+        const float2 ml =
+            __ldcg(reinterpret_cast<const float2*>(warp_part<HDS>(a, c0 + lane, c0 + lane == c1, w) + 32 * HDS + 2 * rr));
+        f = ex2(ml.x - ms);
+        l = ml.y * f;  // a sum is finite or the NaN of a score
+      }
+      // summed in the order of the CTAs, so the bits do not depend on who joins
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        L += __shfl_sync(0xffffffffu, l, i);
+        const float* p = warp_part<HDS>(a, c0 + i, c0 + i == c1, w) + rr * HDS + lane * kPer;
+        float v[kPer];
+        if constexpr (kPer == 4) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
+          v[0] = x.x;
+          v[1] = x.y;
+          v[2] = x.z;
+          v[3] = x.w;
+        } else if constexpr (kPer == 2) {
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+          v[0] = x.x;
+          v[1] = x.y;
+        } else {
+          v[0] = __ldcg(p);
+        }
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) acc[x] += fi == 0.f ? 0.f : v[x] * fi;
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    __nv_bfloat16* dst = out_row(rr) + lane * kPer;
+    uint32_t y[kPer / 2 + 1];
+#pragma unroll
+    for (int x = 0; x + 1 < kPer; x += 2) y[x / 2] = pack_bf16(acc[x] * inv, acc[x + 1] * inv);
+    if constexpr (kPer == 1) {
+      dst[0] = __float2bfloat16_rn(acc[0] * inv);
+    } else if (!a.out_vec) {
+#pragma unroll
+      for (int x = 0; x < kPer; ++x)
+        reinterpret_cast<unsigned short*>(dst)[x] = (unsigned short)(y[x / 2] >> 16 * (x & 1));
+    } else if constexpr (kPer == 4) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(dst) = y[0];
+    }
+  }
+}
+
+template <int HD, int NQ>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                   const __grid_constant__ CUtensorMap tmv, const Args a) {
+  constexpr int NS = n_slots<HD, NQ>();
+  constexpr int kTileBytes = 128 * HD * 2, kHalves = HD / 64;
+  constexpr int HDS = NQ == 1 ? HD / 2 : HD;  // output columns of a softmax thread
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long span_tmp[40];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;                     // [NQ][128 x HD]
+  uint8_t* ring = q_s + NQ * kTileBytes;   // [NS][128 x HD]
+  uint64_t* slot_full = reinterpret_cast<uint64_t*>(ring + NS * kTileBytes);
+  uint64_t* slot_empty = slot_full + NS;
+  uint64_t* guard_full = slot_empty + NS;  // [kGuards] a guarded V tile landed
+  uint64_t* q_full = guard_full + kGuards;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;          // [2]
+  uint64_t* p_half = s_full + 2;           // [2][2]
+  uint64_t* o_full = p_half + 4;           // [2]
+  uint64_t* o_empty = o_full + 2;          // [2] (NQ = 1: one for both outputs)
+  uint64_t* x_bar = o_empty + 2;           // [4] the streams' warps of one lane quarter (NQ = 1)
+  uint64_t* final_bar = x_bar + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  int* poison = abort_flag + 1;            // [kGuards]
+  int* last_bar = poison + kGuards;        // [NS + 1]
+  float* ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(slot_full) + 640);  // [2 segments][2 streams][128][2]
+  volatile int* vabort = abort_flag;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&slot_full[i], 1);
+      mbar_init(&slot_empty[i], 1);
+    }
+    for (int i = 0; i < kGuards; ++i) mbar_init(&guard_full[i], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_half[2 * s], 4);
+      mbar_init(&p_half[2 * s + 1], 4);
+      mbar_init(&o_full[s], 1);
+      mbar_init(&o_empty[s], NQ == 1 ? 8 : 4);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&x_bar[i], 2);
+    mbar_init(final_bar, 1);
+    *abort_flag = 0;
+    for (int i = 0; i <= NS; ++i) last_bar[i] = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  const Span span = my_span<128>(a.rows, a.block_nodes, span_tmp);
+  const int group = a.rows.group, tpt = 128 / group;
+  Walk<128> walk(a.rows, span, a.block_nodes);
+  Segment g;
+  // tiles of a segment that each stream takes
+  auto counts = [&](const Segment& x, int* n) {
+    const int nt = x.t1 - x.t0;
+    if (NQ == 1) {
+      n[0] = (nt + 1) >> 1;
+      n[1] = nt >> 1;
+    } else {
+      n[0] = nt;
+      n[1] = x.block * a.block_nodes + tpt < x.r.nodes ? nt : 0;
+    }
+  };
+  // tiles from here on hold keys that some node may not see
+  auto guard_from = [&](const Segment& x) { return max(x.t0, x.r.slot < 0 ? 0 : x.r.ctx >> 7); };
+  // ring positions of a segment's K and V tiles i of nt, in the order they are
+  // needed: the streams of NQ = 1 start on K tiles 0 and 1
+  auto k_at = [](int i) { return NQ == 1 ? max(2 * i - 1, 0) : 2 * i; };
+  auto v_at = [](int i, int nt) { return NQ == 1 && i < nt - 1 ? 2 * i + 2 : 2 * i + 1; };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8) {
+      // -------------------------------------------------------------- pages
+      const int bs = a.block_size, ppt = 128 / bs, oob = a.num_blocks * a.rows.kv_heads * bs;
+      int c = 0, gd = 0;
+      bool run = true;
+      while (run && walk.next(g)) {
+        const int nt = g.t1 - g.t0, g0 = guard_from(g);
+        const int keys = g.r.ctx + g.r.nodes;
+        const int32_t* table = a.block_table + (int64_t)max(g.r.slot, 0) * a.max_blocks;
+        const int held = g.r.slot >= 0 ? min(a.nblocks[g.r.slot], a.max_blocks) : 0;
+        // lanes hold the pool rows of 32 pages (32 / ppt tiles), the next 32 on their way
+        auto page = [&](int j) -> int {
+          const int pi = g.t0 * ppt + j;
+          if (j >= nt * ppt || pi >= held || pi * bs >= keys) return oob;
+          const int b = __ldg(table + pi);
+          return b >= 0 && b < a.num_blocks ? (b * a.rows.kv_heads + g.hk) * bs : oob;
+        };
+        int chunk_rows[2] = {page(lane), page(32 + lane)};
+        const int tpc = 32 / ppt;  // tiles per chunk
+        int chunk = 0;             // chunk held in chunk_rows[0]; [1] is the next one
+        for (int x = 0; run && x < 2 * nt; ++x) {
+          bool is_v;
+          int i;
+          if (NQ == 1) {
+            // K0 K1 V0 K2 V1 K3 ... V(nt-2) V(nt-1)
+            if (x == 0) {
+              is_v = false;
+              i = 0;
+            } else if (x == 2 * nt - 1) {
+              is_v = true;
+              i = nt - 1;
+            } else {
+              is_v = (x & 1) == 0;
+              i = is_v ? (x - 2) >> 1 : (x + 1) >> 1;
+            }
+          } else {
+            is_v = x & 1;
+            i = x >> 1;
+          }
+          // V runs at most two tiles behind K: its tile is in the chunk held or the next
+          if (i / tpc > chunk && is_v) {
+            ++chunk;
+            chunk_rows[0] = chunk_rows[1];
+            chunk_rows[1] = page(32 * (chunk + 1) + lane);
+          }
+          const int src = (i % tpc) * ppt + (lane & (ppt - 1));
+          const int lo = __shfl_sync(0xffffffffu, chunk_rows[0], src), hi = __shfl_sync(0xffffffffu, chunk_rows[1], src);
+          const int y = i / tpc == chunk ? lo : hi;
+          const int s = c % NS;
+          run = mbar_wait_warp(&slot_empty[s], ((c / NS) & 1) ^ 1, vabort);
+          if (!run) break;
+          const bool guarded = is_v && g.t0 + i >= g0;
+          uint64_t* bar = guarded ? &guard_full[gd % kGuards] : &slot_full[s];
+          if (lane == 0) {
+            last_bar[s] = guarded ? (NS + gd % kGuards) * 2 + ((gd / kGuards) & 1) : s * 2 + ((c / NS) & 1);
+            mbar_expect_tx(bar, kTileBytes);
+          }
+          __syncwarp();
+          if (lane < ppt) {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_2d(ring + s * kTileBytes + h * kHalfBytes + lane * bs * 128, is_v ? &tmv : &tmk, h * 64, y, bar);
+          }
+          __syncwarp();
+          ++c;
+          if (guarded) ++gd;
+        }
+      }
+    } else if (warp == 11) {
+      // -------------------------------------------------------------- queries
+      if (lane == 0) {
+        int nq = 0;
+        while (walk.next(g)) {
+          if (!mbar_wait(q_empty, (nq & 1) ^ 1, vabort)) break;
+          int n[2];
+          counts(g, n);
+          const int tiles = NQ == 2 && n[1] > 0 ? 2 : 1;
+          last_bar[NS] = nq & 1;
+          mbar_expect_tx(q_full, tiles * kHalves * tpt * group * 128);
+          for (int s = 0; s < tiles; ++s)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_3d(q_s + s * kTileBytes + h * kHalfBytes, &tmq, h * 64, g.hk * group,
+                          g.r.n0 + g.block * a.block_nodes + s * tpt, q_full);
+          ++nq;
+        }
+      }
+    } else if (warp == 9) {
+      // -------------------------------------------------------------- products
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = instr_desc(128, 0), idesc_o = instr_desc(HD, 1);
+        constexpr uint32_t kVAtoms = HD == 128 ? (uint32_t)kHalfBytes : 1024u;
+        int c = 0, np[2] = {0, 0}, no[2] = {0, 0}, nq = 0;
+        bool run = true;
+        auto slot_wait = [&](int x) { return mbar_wait(&slot_full[x % NS], (x / NS) & 1, vabort); };
+        auto scores = [&](int s, int x) {
+          const uint32_t qa = su32(q_s + (NQ == 1 ? 0 : s) * kTileBytes), kb = su32(ring + (x % NS) * kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+            mma_ss(tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
+          }
+          mma_commit(&s_full[s]);
+        };
+        // O_s += P_s V once the weights stand there
+        auto values = [&](int s, int x, bool first) -> bool {
+          const uint32_t vb = su32(ring + (x % NS) * kTileBytes);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!mbar_wait(&p_half[2 * s + h], np[s] & 1, vabort)) return false;
+            fence_after();
+#pragma unroll
+            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+              mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
+                     idesc_o, (!first || kk > 0) ? 1u : 0u);
+          }
+          ++np[s];
+          return true;
+        };
+        while (run && walk.next(g)) {
+          int n[2];
+          counts(g, n);
+          const int nt = g.t1 - g.t0;
+          if (!mbar_wait(q_full, nq & 1, vabort)) break;
+          ++nq;
+          if (NQ == 1) {
+            for (int i = 0; run && i < min(nt, 2); ++i) {
+              run = slot_wait(c + k_at(i));
+              if (!run) break;
+              fence_after();
+              scores(i, c + k_at(i));
+              mma_commit(&slot_empty[(c + k_at(i)) % NS]);
+            }
+            if (run && nt <= 2) mma_commit(q_empty);
+            for (int i = 0; run && i < nt; ++i) {
+              const int s = i & 1, vx = c + v_at(i, nt);
+              run = slot_wait(vx);
+              // both outputs of the segment before have been read
+              if (run && i == 0 && no[0] > 0) run = mbar_wait(&o_empty[0], (no[0] - 1) & 1, vabort);
+              if (!run || !values(s, vx, i < 2)) {
+                run = false;
+                break;
+              }
+              mma_commit(&slot_empty[vx % NS]);
+              if (i + 2 < nt) {
+                const int kx = c + k_at(i + 2);
+                run = slot_wait(kx);
+                if (!run) break;
+                fence_after();
+                scores(s, kx);
+                mma_commit(&slot_empty[kx % NS]);
+                if (i + 3 == nt) mma_commit(q_empty);
+              } else {
+                mma_commit(&o_full[s]);
+              }
+            }
+            ++no[0];
+          } else {
+            run = slot_wait(c);
+            if (!run) break;
+            fence_after();
+            for (int s = 0; s < 2; ++s)
+              if (n[s] > 0) scores(s, c);
+            mma_commit(&slot_empty[c % NS]);
+            if (nt == 1) mma_commit(q_empty);
+            for (int i = 0; run && i < nt; ++i) {
+              const int vx = c + v_at(i, nt), kx = c + k_at(i + 1);
+              run = slot_wait(vx) && (i + 1 == nt || slot_wait(kx));
+              for (int s = 0; run && s < 2; ++s) {
+                if (n[s] == 0) continue;
+                if (i == 0 && no[s] > 0) run = mbar_wait(&o_empty[s], (no[s] - 1) & 1, vabort);
+                if (!run || !values(s, vx, i == 0)) {
+                  run = false;
+                  break;
+                }
+                if (i + 1 == nt) {
+                  mma_commit(&o_full[s]);
+                  ++no[s];
+                } else {
+                  fence_after();
+                  scores(s, kx);
+                }
+              }
+              if (!run) break;
+              mma_commit(&slot_empty[vx % NS]);
+              if (i + 1 < nt) mma_commit(&slot_empty[kx % NS]);
+              if (i + 2 == nt) mma_commit(q_empty);
+            }
+          }
+          c += 2 * nt;
+        }
+        mma_commit(final_bar);
+      }
+      __syncwarp();
+    } else {
+      // -------------------------------------------------------------- guard
+      int c = 0, gd = 0, items = 0;
+      bool run = true;
+      while (run && walk.next(g)) {
+        const int nt = g.t1 - g.t0, g0 = guard_from(g);
+        int marks = 0;
+        for (int t = g0; t < g.t1; ++t, ++gd) {
+          if (!mbar_wait_warp(&guard_full[gd % kGuards], (gd / kGuards) & 1, vabort)) {
+            run = false;
+            break;
+          }
+          const int s = (c + v_at(t - g.t0, nt)) % NS;
+          if (tile::clear_nonfinite(reinterpret_cast<uint4*>(ring + s * kTileBytes), kTileBytes / 16))
+            marks |= 1 << min(t - g0, 31);
+          if (lane == 0) {
+            poison[items % kGuards] = marks;
+            mbar_arrive(&slot_full[s]);
+          }
+        }
+        c += 2 * nt;
+        ++items;
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int s = warp >> 2, q4 = warp & 3, r = tid & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16);
+    const int rt = r / group;
+    int nt_done = 0, items = 0, no[2] = {0, 0};
+    bool run = true;
+    while (run && walk.next(g)) {
+      int n[2];
+      counts(g, n);
+      const int item = items++;
+      if (NQ == 2 && n[s] == 0) continue;
+      const int node = g.block * a.block_nodes + (NQ == 2 ? s * tpt : 0) + rt;
+      const bool valid = rt < tpt && node < g.r.nodes;
+      const uint32_t valid_rows = __ballot_sync(0xffffffffu, valid);
+      const int g0 = guard_from(g);
+      const int64_t* mask = a.masks + (int64_t)(g.r.n0 + (valid ? node : 0)) * a.words;
+      auto bits = [&](int key0) { return visible32(mask, a.words, g.r, key0); };
+      tile::RowState row;
+      row.reset();
+      for (int j = 0; j < n[s]; ++j, ++nt_done) {
+        const int t = g.t0 + (NQ == 1 ? 2 * j + s : j);
+        const bool masked = t >= g0;
+        uint32_t vis[4] = {0u, 0u, 0u, 0u};
+        if (masked && valid) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) vis[x] = bits(t * 128 + 32 * x);
+        }
+        if (!mbar_wait_warp(&s_full[s], nt_done & 1, vabort)) {
+          run = false;
+          break;
+        }
+        fence_after();
+        if (!valid_rows) {
+          if (lane == 0) {
+            mbar_arrive(&p_half[2 * s]);
+            mbar_arrive(&p_half[2 * s + 1]);
+          }
+          continue;
+        }
+        tile::softmax_tile<HD>(lane_base, kColS + s * 128, kColO + s * 128, a.scale_log2, j == 0, masked, vis, row,
+                               &p_half[2 * s], &p_half[2 * s + 1]);
+      }
+      if (!run) break;
+      float M = row.m, L = row.l, f0 = 1.f, f1 = 0.f;
+      if (NQ == 1) {
+        // the other stream's statistics of the same row
+        float* x = ml + (item & 1) * 512;
+        *reinterpret_cast<float2*>(x + s * 256 + 2 * r) = make_float2(row.m, row.l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&x_bar[q4]);
+        if (!mbar_wait_warp(&x_bar[q4], item & 1, vabort)) break;
+        const float2 s0 = *reinterpret_cast<const float2*>(x + 2 * r);
+        const float2 s1 = *reinterpret_cast<const float2*>(x + 256 + 2 * r);
+        M = fmaxf(s0.x, s1.x);
+        const float ms = M == -INFINITY ? 0.f : M;
+        f0 = ex2(s0.x - ms);
+        f1 = n[1] > 0 ? ex2(s1.x - ms) : 0.f;
+        L = s0.y * f0 + s1.y * f1;  // a sum is finite or the NaN of a score
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if ((NQ == 1 || x == s) && n[x] > 0) {
+          if (run) run = mbar_wait_warp(&o_full[x], no[x] & 1, vabort);
+          ++no[x];
+        }
+      }
+      if (!run) break;
+      fence_after();
+      const int marks = g0 < g.t1 ? poison[item % kGuards] : 0;
+      const bool whole = g.t0 == 0 && g.t1 == g.tiles;
+      const float inv = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+      auto out_of = [&](int row_in_tile) {
+        const int t = row_in_tile / group;
+        return reinterpret_cast<__nv_bfloat16*>(a.out) +
+               (int64_t)(g.r.n0 + g.block * a.block_nodes + (NQ == 2 ? s * tpt : 0) + t) * a.o_tok +
+               (int64_t)(g.hk * group + row_in_tile - t * group) * a.o_head + (NQ == 1 ? s * HDS : 0);
+      };
+      float* mine = warp_part<HDS>(a, blockIdx.x, g.t0 == 0, warp);
+      __nv_bfloat16* dst = out_of(r);
+#pragma unroll
+      for (int h = 0; h < HDS / 32; ++h) {
+        const int col = (NQ == 1 ? s * HDS : 0) + 32 * h;
+        uint32_t u[32];
+        float* o = reinterpret_cast<float*>(u);
+        if (NQ == 1) {
+          tmem_ld32(lane_base + kColO + col, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = f0 == 0.f ? 0.f : o[x] * f0;
+          if (n[1] > 0) {
+            uint32_t u1[32];
+            tmem_ld32(lane_base + kColO + 128 + col, u1);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] += f1 == 0.f ? 0.f : __uint_as_float(u1[x]) * f1;
+          }
+        } else {
+          tmem_ld32(lane_base + kColO + s * 128 + col, u);
+          tmem_wait_ld();
+        }
+        if (h == HDS / 32 - 1) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[NQ == 1 ? 0 : s]);
+        }
+        if (marks && valid) {
+          const int first = max(g0 * 128, 0), keys = min(g.r.ctx + g.r.nodes, g.t1 * 128);
+#pragma unroll 1
+          for (int key = first; key < keys; ++key) {
+            if (!(marks >> min((key >> 7) - g0, 31) & 1) || !(bits(key & ~31) >> (key & 31) & 1u)) continue;
+            const int bi = key / a.block_size;
+            if (g.r.slot < 0 || bi >= min(a.nblocks[g.r.slot], a.max_blocks)) continue;
+            const int blk = a.block_table[(int64_t)g.r.slot * a.max_blocks + bi];
+            if (blk < 0 || blk >= a.num_blocks) continue;
+            const __nv_bfloat16* v =
+                reinterpret_cast<const __nv_bfloat16*>(a.v_pool) +
+                (((int64_t)blk * a.rows.kv_heads + g.hk) * a.block_size + key % a.block_size) * HD + col;
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const float y = __bfloat162float(v[x]);
+              if (!isfinite(y)) o[x] += y;
+            }
+          }
+        }
+        if (valid && whole) {
+          tile::store_row32(dst + 32 * h, o, inv, a.out_vec);
+        } else if (valid) {
+          float4* p = reinterpret_cast<float4*>(mine + lane * HDS + 32 * h);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) __stcg(p + x, make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]));
+        }
+      }
+      if (whole || !valid_rows) continue;
+      if (valid) __stcg(reinterpret_cast<float2*>(mine + 32 * HDS + 2 * lane), make_float2(M, L));
+      const int c1 = owner(span, g.first), c2 = owner(span, g.first + g.tiles - 1);
+      __threadfence();
+      __syncwarp();
+      int before = 0;
+      if (lane == 0) before = atomicAdd(a.counters + c1 * 8 + warp, 1);
+      if (__shfl_sync(0xffffffffu, before, 0) != c2 - c1) continue;
+      __threadfence();
+      if (lane == 0) a.counters[c1 * 8 + warp] = 0;
+      join_parts<HDS>(a, c1, c2, warp, valid_rows, [&](int rr) { return out_of(32 * q4 + rr); });
+    }
+  }
+
+  __syncthreads();
+  if (*vabort && tid == 0) {
+    atomicOr(a.status, PSE_STATUS_TIMEOUT);
+    for (int i = 0; i < NS; ++i)
+      if (last_bar[i] >= 0) {
+        const int b = last_bar[i] >> 1;
+        mbar_drain(b < NS ? &slot_full[b] : &guard_full[b - NS], last_bar[i] & 1);
+      }
+    if (last_bar[NS] >= 0) mbar_drain(q_full, last_bar[NS]);
+  }
+  if (warp == 9) {
+    if (lane == 0) mbar_drain(final_bar, 0);
+    __syncwarp();
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+Map3Cache g_q_maps;
+TmapCache g_pool_maps;
+
+bool tc_rows(const char* p, int64_t tok, int64_t head, int heads, int hd) {
+  if (heads == 1) head = hd;  // the stride of an axis of one is not used
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= hd && head >= hd &&
+         tok < (1ll << 38) && head < (1ll << 38);
+}
+
+bool tc_eligible(const Args& a, int q_heads) {
+  const int64_t pool_rows = (int64_t)a.num_blocks * a.rows.kv_heads * a.block_size;
+  return (a.hd == 64 || a.hd == 128) &&
+         (a.block_size == 16 || a.block_size == 32 || a.block_size == 64 || a.block_size == 128) && a.num_blocks > 0 &&
+         a.scale_log2 > 0.f && (reinterpret_cast<uintptr_t>(a.k_pool) | reinterpret_cast<uintptr_t>(a.v_pool)) % 16 == 0 &&
+         pool_rows + a.block_size < (1ll << 31) && tc_rows(a.q, a.q_tok, a.q_head, q_heads, a.hd);
+}
+
+template <int HD, int NQ>
+int launch_tc(Args& a, int q_heads, cudaStream_t s) {
+  auto kern = tree_tc_kernel<HD, NQ>;
+  constexpr size_t smem = tc_smem_bytes<HD, NQ>();
+  static_assert(smem + 320 <= 227 * 1024, "shared memory");
+  static const cudaError_t opt = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (opt != cudaSuccess) return (int)opt;
+  const int tpt = 128 / a.rows.group;
+  a.block_nodes = NQ * tpt;
+  CUtensorMap mq, mk, mv;
+  int rc = g_q_maps.get(Map3Key{reinterpret_cast<uint64_t>(a.q), (uint64_t)HD, (uint64_t)q_heads,
+                                (uint64_t)a.rows.n_nodes, (uint64_t)(q_heads == 1 ? HD : a.q_head) * 2,
+                                (uint64_t)a.q_tok * 2, (uint32_t)a.rows.group, (uint32_t)tpt},
+                        &mq);
+  const uint64_t pool_rows = (uint64_t)a.num_blocks * a.rows.kv_heads * a.block_size;
+  if (rc == 0) rc = g_pool_maps.get(a.k_pool, HD, pool_rows, HD * 2, 64u, a.block_size, PSE_EINVAL, &mk);
+  if (rc == 0) rc = g_pool_maps.get(a.v_pool, HD, pool_rows, HD * 2, 64u, a.block_size, PSE_EINVAL, &mv);
+  if (rc) return rc;
+  const cudaError_t e = launch_pdl(kern, dim3(kNumSMs), dim3(kTcThreads), smem, s, mq, mk, mv, a);
+  return e == cudaSuccess ? PSE_OK : (int)e;
+}
+
+template <int HD>
+int tc_attention(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
+  return max_nodes > 128 / a.rows.group ? launch_tc<HD, 2>(a, q_heads, s) : launch_tc<HD, 1>(a, q_heads, s);
 }
 
 // Node ancestors: bit m of node n's mask for m = n and every node on the way
@@ -231,8 +851,9 @@ extern "C" int pse_tree_masks(const int32_t* parents, const int32_t* node_off, i
 
 extern "C" size_t pse_token_tree_workspace(int32_t head_dim) {
   if (head_dim <= 0) return 0;
-  // two partial results of up to 64 rows per CTA
-  return (size_t)tree::kCounterBytes + (size_t)tree::kMaxCtas * 2 * 64 * (head_dim + 2) * 4;
+  // two partial results per CTA: of 64 rows on the CUDA cores, of 256 on the tensor cores
+  const size_t simt = (size_t)tree::kMaxCtas * 64, tc = (size_t)kNumSMs * 256;
+  return (size_t)tree::kCounterBytes + (head_dim <= 128 && tc > simt ? tc : simt) * 2 * (head_dim + 2) * 4;
 }
 
 extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,
@@ -282,6 +903,10 @@ extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse
   a.counters = (int32_t*)workspace;
   a.parts = (float*)((char*)workspace + tree::kCounterBytes);
   a.status = st.status;
+  a.out_vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
+  if (kv.dtype == PSE_BF16 && tree::tc_eligible(a, q.heads))
+    return a.hd == 64 ? tree::tc_attention<64>(a, q.heads, max_nodes, (cudaStream_t)stream)
+                      : tree::tc_attention<128>(a, q.heads, max_nodes, (cudaStream_t)stream);
   return kv.dtype == PSE_BF16 ? tree::simt_attention<__nv_bfloat16>(a, max_nodes, (cudaStream_t)stream)
                               : tree::simt_attention<float>(a, max_nodes, (cudaStream_t)stream);
 }
