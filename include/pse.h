@@ -458,9 +458,9 @@ int pse_tree_masks(const int32_t *parents, const int32_t *node_off, int32_t rows
  * table cannot hold.  max_nodes bounds the rows' node counts (it picks the
  * kernel's shape; max_nodes <= 64 words).  ctx, slots and node_off are read on
  * the device only, so the call can be captured and replayed with other values.
- * workspace: pse_token_tree_workspace() bytes, 16-byte aligned, the first 8192
- * of them zero before the first call and zero again after every call; calls
- * that share one must not overlap on the GPU. */
+ * workspace: pse_token_tree_workspace() bytes, 16-byte aligned, written before
+ * it is read (what stands in it does not matter); calls that share one must
+ * not overlap on the GPU. */
 int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,
                              const int32_t *slots, const int32_t *ctx, const int32_t *node_off, int32_t rows,
                              int32_t n_nodes, int32_t max_nodes, const int64_t *masks, int32_t words, float scale,

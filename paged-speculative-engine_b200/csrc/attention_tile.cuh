@@ -49,13 +49,17 @@ __device__ __forceinline__ void softmax_tile(uint32_t lane_base, uint32_t s_col,
   }
   float m4[4];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) m4[x] = fmaxf(s[x], s[x + 4]);
+  for (int x = 0; x < 4; ++x) m4[x] = fmax3_nan(s[x], s[x + 4], s[x + 8]);
 #pragma unroll
-  for (int c = 8; c < kKeys; c += 8) {
+  for (int c = 12; c + 8 <= kKeys; c += 8) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) m4[x] = fmaxf(fmaxf(m4[x], s[c + x]), s[c + 4 + x]);
+    for (int x = 0; x < 4; ++x) m4[x] = fmax3_nan(m4[x], s[c + x], s[c + 4 + x]);
   }
-  const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) m4[x] = fmax3_nan(m4[x], s[kKeys - 4 + x], s[kKeys - 4 + x]);
+  const float mx = fmax3_nan(fmax3_nan(m4[0], m4[1], m4[2]), m4[3], m4[3]) * sl2;
+  // a NaN or +inf among the scores: the row's result is NaN
+  if (!(mx < INFINITY)) row.l = __int_as_float(0x7fffffff);
   float corr = 1.f;
   if (mx > row.m + 8.f) {
     corr = ex2(row.m - mx);  // 0 from -inf

@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   int* last_bar = poison + kGuards;        // [NS + 1] per slot (and Q): barrier and parity of its last copy
   volatile int* vabort = abort_flag;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&slot_full[i], 1);
@@ -289,7 +290,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     } else if (warp == 9) {
       // -------------------------------------------------------------- products
-      if (lane == 0) {
+      {
+        const uint32_t el = elect_one();
         constexpr uint32_t idesc_s = instr_desc(128, 0), idesc_o = instr_desc(HD, 1);
         constexpr uint32_t kVAtoms = HD == 128 ? (uint32_t)kHalfBytes : 1024u;
         int c = 0;             // slots used by earlier tiles: K of tile j at c + 2 j, V at c + 2 j + 1
@@ -297,26 +299,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int no[2] = {0, 0};    // items finished per stream
         int nq = 0;
         bool run = true;
-        auto slot_wait = [&](int x) { return mbar_wait(&slot_full[x % NS], (x / NS) & 1, vabort); };
+        auto slot_wait = [&](int x) { return mbar_wait_warp(&slot_full[x % NS], (x / NS) & 1, vabort); };
         auto scores = [&](int s, int x) {
           const uint32_t qa = su32(q_s + s * kTileBytes), kb = su32(ring + (x % NS) * kTileBytes);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-            mma_ss(tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
+            mma_ss(el, tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
           }
-          mma_commit(&s_full[s]);
+          mma_commit(el, &s_full[s]);
         };
         for (int e = e0; run && e < e1; ++e) {
           const TcItem it = decode(a, e, tpt);
           if (it.n_max == 0) continue;
-          if (!mbar_wait(q_full, nq & 1, vabort) || !slot_wait(c)) break;
+          if (!mbar_wait_warp(q_full, nq & 1, vabort) || !slot_wait(c)) break;
           ++nq;
           fence_after();
           for (int s = 0; s < 2; ++s)
             if (it.n[s] > 0) scores(s, c);
-          mma_commit(&slot_empty[c % NS]);
-          if (it.n_max == 1) mma_commit(q_empty);
+          mma_commit(el, &slot_empty[c % NS]);
+          if (it.n_max == 1) mma_commit(el, q_empty);
           for (int j = 0; run && j < it.n_max; ++j) {
             const int kx = c + 2 * (j + 1), vx = c + 2 * j + 1;
             bool v_here = false, k_here = false;
@@ -324,22 +326,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (j >= it.n[s]) continue;
               if (!v_here) run = slot_wait(vx);
               v_here = true;
-              if (run && j == 0 && no[s] > 0) run = mbar_wait(&o_empty[s], (no[s] - 1) & 1, vabort);
+              if (run && j == 0 && no[s] > 0) run = mbar_wait_warp(&o_empty[s], (no[s] - 1) & 1, vabort);
               const uint32_t vb = su32(ring + (vx % NS) * kTileBytes);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                if (run) run = mbar_wait(&p_half[2 * s + h], np[s] & 1, vabort);
+                if (run) run = mbar_wait_warp(&p_half[2 * s + h], np[s] & 1, vabort);
                 if (!run) break;
                 fence_after();
 #pragma unroll
                 for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                  mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
+                  mma_ts(el, tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
                          idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
               }
               if (!run) break;
               ++np[s];
               if (j + 1 == it.n[s]) {
-                mma_commit(&o_full[s]);
+                mma_commit(el, &o_full[s]);
                 ++no[s];
               } else {
                 if (!k_here) run = slot_wait(kx);
@@ -350,17 +352,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               }
             }
             if (!run) break;
-            mma_commit(&slot_empty[vx % NS]);
+            mma_commit(el, &slot_empty[vx % NS]);
             if (k_here) {
-              mma_commit(&slot_empty[kx % NS]);
-              if (j + 2 == it.n_max) mma_commit(q_empty);
+              mma_commit(el, &slot_empty[kx % NS]);
+              if (j + 2 == it.n_max) mma_commit(el, q_empty);
             }
           }
           c += 2 * it.n_max;
         }
-        mma_commit(final_bar);
+        mma_commit(el, final_bar);
       }
-      __syncwarp();
     } else if (warp == 10) {
       // -------------------------------------------------------------- guard
       int c = 0, g = 0, items = 0;

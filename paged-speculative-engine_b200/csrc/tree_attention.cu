@@ -14,8 +14,9 @@
 namespace pse {
 namespace tree {
 
+struct Cut;
 constexpr int kMaxCtas = 2 * kNumSMs;
-constexpr int kCounterBytes = 8192;  // a counter per CTA, or per softmax warp of one
+constexpr size_t kCutBytes = 8192;  // a Cut per CTA
 
 struct Args {
   Rows rows;
@@ -32,16 +33,89 @@ struct Args {
   int words;
   int block_nodes;
   float scale_log2;
-  int32_t* counters;  // [kMaxCtas], zero between calls
-  float* parts;       // [ctas][2][block rows][hd + 2]
+  Cut* cuts;  // [ctas]
+  float* parts;      // [ctas][2][part_rows][hd + 2]
+  int part_rows;
   int32_t* status;
   bool out_vec;  // output rows are 16-byte aligned
 };
 
-// Which of its CTA's two partial results a segment writes: the first segment's
-// item may be cut at its start, the last one's at its end.
-__device__ __forceinline__ float* part(const Args& a, int cta, bool starts_item, int rows) {
-  return a.parts + ((int64_t)cta * 2 + (starts_item ? 1 : 0)) * rows * (a.hd + 2);
+// Partial results of cut items: per CTA two blocks of `part_rows` rows of hd
+// columns, then a (maximum, sum) per row.  A CTA's first segment, if it begins
+// inside an item, uses the first block; a segment that begins an item and does
+// not end it, necessarily the CTA's last, uses the second.
+__device__ __forceinline__ float* part(const Args& a, int cta, bool starts_item) {
+  return a.parts + ((int64_t)cta * 2 + (starts_item ? 1 : 0)) * a.part_rows * (a.hd + 2);
+}
+__device__ __forceinline__ float* part_row(const Args& a, float* block, int r) { return block + (int64_t)r * a.hd; }
+__device__ __forceinline__ float* part_stats(const Args& a, float* block, int r) {
+  return block + (int64_t)a.part_rows * a.hd + 2 * r;
+}
+
+// What the join needs of the item that CTA c begins and does not end.
+struct Cut {
+  int last;    // the item's last CTA (-1: CTA c cuts nothing)
+  int node0;   // its first query node
+  int nodes;   // and their number
+  int hk;
+};
+
+// A warp per row of a cut item, lanes over the columns: the parts are summed in
+// the order of their CTAs.
+template <typename T, int PER>
+__global__ void join_kernel(const Args a, int tile_rows, int tile_pitch) {
+  pdl_wait();
+  const int4 x = *reinterpret_cast<const int4*>(a.cuts + blockIdx.x);
+  const int c1 = blockIdx.x, c2 = x.x, node0 = x.y, hk = x.w, group = a.rows.group, hd = a.hd;
+  const int row = blockIdx.y * (blockDim.x / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (c2 < 0 || row >= x.z * group) return;
+  const int r = row / tile_rows * tile_pitch + row % tile_rows;
+  float M = -INFINITY;
+  for (int c = c1 + lane; c <= c2; c += 32) M = fmaxf(M, part_stats(a, part(a, c, c == c1), r)[0]);
+  M = warp_max(M);
+  const float ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f, acc[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  for (int c0 = c1; c0 <= c2; c0 += 32) {
+    const int n = min(32, c2 + 1 - c0);
+    float f = 0.f, l = 0.f;
+    if (lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(part_stats(a, part(a, c0 + lane, c0 + lane == c1), r));
+      f = exp2f(ml.x - ms);
+      l = ml.y * f;  // a sum is finite or the NaN of a score
+    }
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      L += __shfl_sync(0xffffffffu, l, i);
+      const float* p = part_row(a, part(a, c0 + i, c0 + i == c1), r);
+#pragma unroll
+      for (int y = 0; y < PER; ++y) {
+        const int d = lane + 32 * y;
+        if (d < hd) acc[y] += fi == 0.f ? 0.f : p[d] * fi;
+      }
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(node0 + row / group) * a.o_tok +
+           (int64_t)(hk * group + row % group) * a.o_head;
+#pragma unroll
+  for (int y = 0; y < PER; ++y) {
+    const int d = lane + 32 * y;
+    if (d < hd) dst[d] = from_f32<T>(acc[y] * inv);
+  }
+}
+
+template <typename T>
+int launch_join(const Args& a, int ctas, int max_nodes, int tile_rows, int tile_pitch, cudaStream_t s) {
+  const int rows = (max_nodes < a.block_nodes ? max_nodes : a.block_nodes) * a.rows.group;
+  const int warps = rows < 16 ? rows : 16;
+  const dim3 grid(ctas, ceil_div(rows, warps)), block(32 * warps);
+  const cudaError_t e = a.hd <= 64    ? launch_pdl(join_kernel<T, 2>, grid, block, 0, s, a, tile_rows, tile_pitch)
+                        : a.hd <= 128 ? launch_pdl(join_kernel<T, 4>, grid, block, 0, s, a, tile_rows, tile_pitch)
+                                      : launch_pdl(join_kernel<T, 8>, grid, block, 0, s, a, tile_rows, tile_pitch);
+  return e == cudaSuccess ? PSE_OK : (int)e;
 }
 
 // ---------------------------------------------------------------- CUDA cores
@@ -49,10 +123,9 @@ template <typename T, int RPT, int NC>
 __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a) {
   extern __shared__ float smem[];
   __shared__ long long tmp[40];
-  __shared__ int last;
   constexpr int BQ = 16 * RPT, TILE = simt::BK;
   const Span span = my_span<TILE>(a.rows, a.block_nodes, tmp);
-  if ((int)blockIdx.x >= span.ctas) return;
+  Cut cut{-1, 0, 0, 0};
   simt::Tile<RPT, NC> t;
   t.init(smem, a.hd);
   const int group = a.rows.group, hd = a.hd;
@@ -108,7 +181,9 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
       return out + (int64_t)(g.r.n0 + node0 + r / group) * a.o_tok + (int64_t)(g.hk * group + r % group) * a.o_head;
     };
     const bool whole = g.t0 == 0 && g.t1 == g.tiles;
-    float* mine = part(a, blockIdx.x, g.t0 == 0, BQ);
+    float* mine = part(a, blockIdx.x, g.t0 == 0);
+    if (g.t0 == 0 && !whole)
+      cut = Cut{owner(span, g.first + g.tiles - 1), g.r.n0 + node0, min(a.block_nodes, g.r.nodes - node0), g.hk};
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       const float L = t.row_sum(i);
@@ -127,40 +202,16 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
           x.w *= inv;
           simt::store4(out_row(r) + d, hd - d, x);
         } else {
-          simt::store4(mine + (int64_t)r * (hd + 2) + d, hd - d, x);
+          simt::store4(part_row(a, mine, r) + d, hd - d, x);
         }
       }
       if (!whole && t.tx == 0) {
-        mine[(int64_t)r * (hd + 2) + hd] = t.m[i];
-        mine[(int64_t)r * (hd + 2) + hd + 1] = L;
+        part_stats(a, mine, r)[0] = t.m[i];
+        part_stats(a, mine, r)[1] = L;
       }
     }
-    if (whole) continue;
-    const int c1 = owner(span, g.first), c2 = owner(span, g.first + g.tiles - 1);
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.counters + c1, 1) == c2 - c1;
-    __syncthreads();
-    if (!last) continue;
-    __threadfence();
-    if (threadIdx.x == 0) a.counters[c1] = 0;
-    for (int e = threadIdx.x; e < nr * hd; e += simt::kThreads) {
-      const int r = e / hd, d = e - r * hd;
-      float M = -INFINITY;
-      for (int c = c1; c <= c2; ++c)
-        M = fmaxf(M, __ldcg(part(a, c, c == c1, BQ) + (int64_t)r * (hd + 2) + hd));
-      const float ms = M == -INFINITY ? 0.f : M;
-      float L = 0.f, x = 0.f;
-      for (int c = c1; c <= c2; ++c) {
-        const float* p = part(a, c, c == c1, BQ) + (int64_t)r * (hd + 2);
-        const float f = exp2f(__ldcg(p + hd) - ms);
-        L += __ldcg(p + hd + 1) * f;  // a sum is finite or the NaN of a score
-        if (f != 0.f) x += __ldcg(p + d) * f;
-      }
-      out_row(r)[d] = from_f32<T>(L == 0.f ? 0.f : x / L);
-    }
-    __syncthreads();
   }
+  if (threadIdx.x == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(cut.last, cut.node0, cut.nodes, cut.hk);
 }
 
 int simt_rows(int rows) { return rows <= 16 ? 1 : 4; }
@@ -188,7 +239,9 @@ template <typename T>
 int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
   const int rpt = simt_rows(max_nodes * a.rows.group);
   a.block_nodes = 16 * rpt / a.rows.group;
-  return rpt == 1 ? simt_nc<T, 1>(a, kMaxCtas, s) : simt_nc<T, 4>(a, kMaxCtas, s);
+  a.part_rows = 16 * rpt;
+  const int rc = rpt == 1 ? simt_nc<T, 1>(a, kMaxCtas, s) : simt_nc<T, 4>(a, kMaxCtas, s);
+  return rc == PSE_OK ? launch_join<T>(a, kMaxCtas, max_nodes, a.part_rows, a.part_rows, s) : rc;
 }
 
 // ---------------------------------------------------------------- tensor cores
@@ -204,7 +257,7 @@ int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
 // Either way one stream's softmax runs beside the other's products.  Warps:
 //   0-3, 4-7  the streams' softmax (attention_tile.cuh), a thread per row
 //   8         K and V pages by TMA into a ring of 128-key slots
-//   9         one thread issues the products
+//   9         the products
 //   10        clears V tiles that hold nodes (or what stands after them) of
 //             infinities and NaN before the product, as in prompt_attention.cu
 //   11        Q tiles, so that the ring runs on into the next segment
@@ -221,80 +274,6 @@ __host__ __device__ constexpr int n_slots() { return HD == 128 ? 5 : 10; }
 template <int HD, int NQ>
 constexpr size_t tc_smem_bytes() {
   return 1024 + (size_t)(NQ + n_slots<HD, NQ>()) * 128 * HD * 2 + 640 + (NQ == 1 ? 4096 : 0);
-}
-
-// One softmax warp's partial results: 32 rows of HDS columns, then 32 (maximum, sum).
-template <int HDS>
-__device__ __forceinline__ float* warp_part(const Args& a, int cta, bool starts_item, int w) {
-  return a.parts + (((int64_t)cta * 2 + (starts_item ? 1 : 0)) * 8 + w) * 32 * (HDS + 2);
-}
-
-// The last warp to arrive joins the parts of its 32 rows, lanes over the columns.
-template <int HDS, typename F>
-__device__ __forceinline__ void join_parts(const Args& a, int c1, int c2, int w, uint32_t rows, F out_row) {
-  constexpr int kPer = HDS / 32;
-  const int lane = threadIdx.x & 31;
-  while (rows) {
-    const int rr = __ffs(rows) - 1;
-    rows &= rows - 1;
-    float M = -INFINITY;
-    for (int c = c1 + lane; c <= c2; c += 32)
-      M = fmaxf(M, __ldcg(warp_part<HDS>(a, c, c == c1, w) + 32 * HDS + 2 * rr));
-    M = warp_max(M);
-    const float ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[kPer];
-#pragma unroll
-    for (int x = 0; x < kPer; ++x) acc[x] = 0.f;
-    for (int c0 = c1; c0 <= c2; c0 += 32) {
-      const int n = min(32, c2 + 1 - c0);
-      float f = 0.f, l = 0.f;
-      if (lane < n) {
-        const float2 ml =
-            __ldcg(reinterpret_cast<const float2*>(warp_part<HDS>(a, c0 + lane, c0 + lane == c1, w) + 32 * HDS + 2 * rr));
-        f = ex2(ml.x - ms);
-        l = ml.y * f;  // a sum is finite or the NaN of a score
-      }
-      // summed in the order of the CTAs, so the bits do not depend on who joins
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        L += __shfl_sync(0xffffffffu, l, i);
-        const float* p = warp_part<HDS>(a, c0 + i, c0 + i == c1, w) + rr * HDS + lane * kPer;
-        float v[kPer];
-        if constexpr (kPer == 4) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
-          v[0] = x.x;
-          v[1] = x.y;
-          v[2] = x.z;
-          v[3] = x.w;
-        } else if constexpr (kPer == 2) {
-          const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
-          v[0] = x.x;
-          v[1] = x.y;
-        } else {
-          v[0] = __ldcg(p);
-        }
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) acc[x] += fi == 0.f ? 0.f : v[x] * fi;
-      }
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    __nv_bfloat16* dst = out_row(rr) + lane * kPer;
-    uint32_t y[kPer / 2 + 1];
-#pragma unroll
-    for (int x = 0; x + 1 < kPer; x += 2) y[x / 2] = pack_bf16(acc[x] * inv, acc[x + 1] * inv);
-    if constexpr (kPer == 1) {
-      dst[0] = __float2bfloat16_rn(acc[0] * inv);
-    } else if (!a.out_vec) {
-#pragma unroll
-      for (int x = 0; x < kPer; ++x)
-        reinterpret_cast<unsigned short*>(dst)[x] = (unsigned short)(y[x / 2] >> 16 * (x & 1));
-    } else if constexpr (kPer == 4) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(y[0], y[1]);
-    } else {
-      *reinterpret_cast<uint32_t*>(dst) = y[0];
-    }
-  }
 }
 
 template <int HD, int NQ>
@@ -327,7 +306,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   float* ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(slot_full) + 640);  // [2 segments][2 streams][128][2]
   volatile int* vabort = abort_flag;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&slot_full[i], 1);
@@ -471,31 +451,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     } else if (warp == 9) {
       // -------------------------------------------------------------- products
-      if (lane == 0) {
+      {
+        const uint32_t el = elect_one();
         constexpr uint32_t idesc_s = instr_desc(128, 0), idesc_o = instr_desc(HD, 1);
         constexpr uint32_t kVAtoms = HD == 128 ? (uint32_t)kHalfBytes : 1024u;
         int c = 0, np[2] = {0, 0}, no[2] = {0, 0}, nq = 0;
         bool run = true;
-        auto slot_wait = [&](int x) { return mbar_wait(&slot_full[x % NS], (x / NS) & 1, vabort); };
+        auto slot_wait = [&](int x) { return mbar_wait_warp(&slot_full[x % NS], (x / NS) & 1, vabort); };
         auto scores = [&](int s, int x) {
           const uint32_t qa = su32(q_s + (NQ == 1 ? 0 : s) * kTileBytes), kb = su32(ring + (x % NS) * kTileBytes);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-            mma_ss(tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
+            mma_ss(el, tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
           }
-          mma_commit(&s_full[s]);
+          mma_commit(el, &s_full[s]);
         };
         // O_s += P_s V once the weights stand there
         auto values = [&](int s, int x, bool first) -> bool {
           const uint32_t vb = su32(ring + (x % NS) * kTileBytes);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (!mbar_wait(&p_half[2 * s + h], np[s] & 1, vabort)) return false;
+            if (!mbar_wait_warp(&p_half[2 * s + h], np[s] & 1, vabort)) return false;
             fence_after();
 #pragma unroll
             for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-              mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
+              mma_ts(el, tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
                      idesc_o, (!first || kk > 0) ? 1u : 0u);
           }
           ++np[s];
@@ -505,7 +486,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           int n[2];
           counts(g, n);
           const int nt = g.t1 - g.t0;
-          if (!mbar_wait(q_full, nq & 1, vabort)) break;
+          if (!mbar_wait_warp(q_full, nq & 1, vabort)) break;
           ++nq;
           if (NQ == 1) {
             for (int i = 0; run && i < min(nt, 2); ++i) {
@@ -513,29 +494,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (!run) break;
               fence_after();
               scores(i, c + k_at(i));
-              mma_commit(&slot_empty[(c + k_at(i)) % NS]);
+              mma_commit(el, &slot_empty[(c + k_at(i)) % NS]);
             }
-            if (run && nt <= 2) mma_commit(q_empty);
+            if (run && nt <= 2) mma_commit(el, q_empty);
             for (int i = 0; run && i < nt; ++i) {
               const int s = i & 1, vx = c + v_at(i, nt);
               run = slot_wait(vx);
               // both outputs of the segment before have been read
-              if (run && i == 0 && no[0] > 0) run = mbar_wait(&o_empty[0], (no[0] - 1) & 1, vabort);
+              if (run && i == 0 && no[0] > 0) run = mbar_wait_warp(&o_empty[0], (no[0] - 1) & 1, vabort);
               if (!run || !values(s, vx, i < 2)) {
                 run = false;
                 break;
               }
-              mma_commit(&slot_empty[vx % NS]);
+              mma_commit(el, &slot_empty[vx % NS]);
               if (i + 2 < nt) {
                 const int kx = c + k_at(i + 2);
                 run = slot_wait(kx);
                 if (!run) break;
                 fence_after();
                 scores(s, kx);
-                mma_commit(&slot_empty[kx % NS]);
-                if (i + 3 == nt) mma_commit(q_empty);
+                mma_commit(el, &slot_empty[kx % NS]);
+                if (i + 3 == nt) mma_commit(el, q_empty);
               } else {
-                mma_commit(&o_full[s]);
+                mma_commit(el, &o_full[s]);
               }
             }
             ++no[0];
@@ -543,22 +524,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             run = slot_wait(c);
             if (!run) break;
             fence_after();
+#pragma unroll
             for (int s = 0; s < 2; ++s)
               if (n[s] > 0) scores(s, c);
-            mma_commit(&slot_empty[c % NS]);
-            if (nt == 1) mma_commit(q_empty);
+            mma_commit(el, &slot_empty[c % NS]);
+            if (nt == 1) mma_commit(el, q_empty);
             for (int i = 0; run && i < nt; ++i) {
               const int vx = c + v_at(i, nt), kx = c + k_at(i + 1);
               run = slot_wait(vx) && (i + 1 == nt || slot_wait(kx));
-              for (int s = 0; run && s < 2; ++s) {
+  #pragma unroll
+            for (int s = 0; run && s < 2; ++s) {
                 if (n[s] == 0) continue;
-                if (i == 0 && no[s] > 0) run = mbar_wait(&o_empty[s], (no[s] - 1) & 1, vabort);
+                if (i == 0 && no[s] > 0) run = mbar_wait_warp(&o_empty[s], (no[s] - 1) & 1, vabort);
                 if (!run || !values(s, vx, i == 0)) {
                   run = false;
                   break;
                 }
                 if (i + 1 == nt) {
-                  mma_commit(&o_full[s]);
+                  mma_commit(el, &o_full[s]);
                   ++no[s];
                 } else {
                   fence_after();
@@ -566,16 +549,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
               }
               if (!run) break;
-              mma_commit(&slot_empty[vx % NS]);
-              if (i + 1 < nt) mma_commit(&slot_empty[kx % NS]);
-              if (i + 2 == nt) mma_commit(q_empty);
+              mma_commit(el, &slot_empty[vx % NS]);
+              if (i + 1 < nt) mma_commit(el, &slot_empty[kx % NS]);
+              if (i + 2 == nt) mma_commit(el, q_empty);
             }
           }
           c += 2 * nt;
         }
-        mma_commit(final_bar);
+        mma_commit(el, final_bar);
       }
-      __syncwarp();
     } else {
       // -------------------------------------------------------------- guard
       int c = 0, gd = 0, items = 0;
@@ -607,6 +589,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16);
     const int rt = r / group;
     int nt_done = 0, items = 0, no[2] = {0, 0};
+    Cut cut{-1, 0, 0, 0};
     bool run = true;
     while (run && walk.next(g)) {
       int n[2];
@@ -679,7 +662,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                (int64_t)(g.r.n0 + g.block * a.block_nodes + (NQ == 2 ? s * tpt : 0) + t) * a.o_tok +
                (int64_t)(g.hk * group + row_in_tile - t * group) * a.o_head + (NQ == 1 ? s * HDS : 0);
       };
-      float* mine = warp_part<HDS>(a, blockIdx.x, g.t0 == 0, warp);
+      float* mine = part(a, blockIdx.x, g.t0 == 0);
+      const int prow = (NQ == 2 ? s * 128 : 0) + r;
+      if (g.t0 == 0 && !whole)
+        cut = Cut{owner(span, g.first + g.tiles - 1), g.r.n0 + g.block * a.block_nodes,
+                  min(a.block_nodes, g.r.nodes - g.block * a.block_nodes), g.hk};
       __nv_bfloat16* dst = out_of(r);
 #pragma unroll
       for (int h = 0; h < HDS / 32; ++h) {
@@ -729,23 +716,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (valid && whole) {
           tile::store_row32(dst + 32 * h, o, inv, a.out_vec);
         } else if (valid) {
-          float4* p = reinterpret_cast<float4*>(mine + lane * HDS + 32 * h);
+          float4* p = reinterpret_cast<float4*>(part_row(a, mine, prow) + col);
 #pragma unroll
           for (int x = 0; x < 8; ++x) __stcg(p + x, make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]));
         }
       }
-      if (whole || !valid_rows) continue;
-      if (valid) __stcg(reinterpret_cast<float2*>(mine + 32 * HDS + 2 * lane), make_float2(M, L));
-      const int c1 = owner(span, g.first), c2 = owner(span, g.first + g.tiles - 1);
-      __threadfence();
-      __syncwarp();
-      int before = 0;
-      if (lane == 0) before = atomicAdd(a.counters + c1 * 8 + warp, 1);
-      if (__shfl_sync(0xffffffffu, before, 0) != c2 - c1) continue;
-      __threadfence();
-      if (lane == 0) a.counters[c1 * 8 + warp] = 0;
-      join_parts<HDS>(a, c1, c2, warp, valid_rows, [&](int rr) { return out_of(32 * q4 + rr); });
+      if (!whole && valid && (NQ == 2 || s == 0))
+        __stcg(reinterpret_cast<float2*>(part_stats(a, mine, prow)), make_float2(M, L));
     }
+    if (tid == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(cut.last, cut.node0, cut.nodes, cut.hk);
   }
 
   __syncthreads();
@@ -784,7 +763,7 @@ bool tc_eligible(const Args& a, int q_heads) {
 }
 
 template <int HD, int NQ>
-int launch_tc(Args& a, int q_heads, cudaStream_t s) {
+int launch_tc(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
   auto kern = tree_tc_kernel<HD, NQ>;
   constexpr size_t smem = tc_smem_bytes<HD, NQ>();
   static_assert(smem + 320 <= 227 * 1024, "shared memory");
@@ -801,13 +780,16 @@ int launch_tc(Args& a, int q_heads, cudaStream_t s) {
   if (rc == 0) rc = g_pool_maps.get(a.k_pool, HD, pool_rows, HD * 2, 64u, a.block_size, PSE_EINVAL, &mk);
   if (rc == 0) rc = g_pool_maps.get(a.v_pool, HD, pool_rows, HD * 2, 64u, a.block_size, PSE_EINVAL, &mv);
   if (rc) return rc;
+  a.part_rows = 128 * NQ;
   const cudaError_t e = launch_pdl(kern, dim3(kNumSMs), dim3(kTcThreads), smem, s, mq, mk, mv, a);
-  return e == cudaSuccess ? PSE_OK : (int)e;
+  if (e != cudaSuccess) return (int)e;
+  return launch_join<__nv_bfloat16>(a, kNumSMs, max_nodes, tpt * a.rows.group, 128, s);
 }
 
 template <int HD>
 int tc_attention(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
-  return max_nodes > 128 / a.rows.group ? launch_tc<HD, 2>(a, q_heads, s) : launch_tc<HD, 1>(a, q_heads, s);
+  return max_nodes > 128 / a.rows.group ? launch_tc<HD, 2>(a, q_heads, max_nodes, s)
+                                        : launch_tc<HD, 1>(a, q_heads, max_nodes, s);
 }
 
 // Node ancestors: bit m of node n's mask for m = n and every node on the way
@@ -853,7 +835,7 @@ extern "C" size_t pse_token_tree_workspace(int32_t head_dim) {
   if (head_dim <= 0) return 0;
   // two partial results per CTA: of 64 rows on the CUDA cores, of 256 on the tensor cores
   const size_t simt = (size_t)tree::kMaxCtas * 64, tc = (size_t)kNumSMs * 256;
-  return (size_t)tree::kCounterBytes + (head_dim <= 128 && tc > simt ? tc : simt) * 2 * (head_dim + 2) * 4;
+  return tree::kCutBytes + (head_dim <= 128 && tc > simt ? tc : simt) * 2 * (head_dim + 2) * 4;
 }
 
 extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,
@@ -900,8 +882,8 @@ extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse
   a.masks = masks;
   a.words = words;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.counters = (int32_t*)workspace;
-  a.parts = (float*)((char*)workspace + tree::kCounterBytes);
+  a.cuts = (tree::Cut*)workspace;
+  a.parts = (float*)((char*)workspace + tree::kCutBytes);
   a.status = st.status;
   a.out_vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
   if (kv.dtype == PSE_BF16 && tree::tc_eligible(a, q.heads))

@@ -7,9 +7,10 @@
 // number of tiles (within one) whatever the lengths are, and nothing about
 // them has to be known on the host.  An item whose tiles all fall to one CTA
 // is finished there.  An item cut by CTA boundaries leaves one partial result
-// per CTA (maximum, sum and unnormalised output) in the workspace, and the
-// last of its CTAs to arrive joins them in the order of the CTAs: the order of
-// arrival changes who joins, never the result.
+// per CTA (maximum, sum and unnormalised output) in the workspace, which a
+// second, small kernel joins in the order of the CTAs.  (Joining by the last CTA
+// to arrive saves that launch but leaves the rows of an item to one warp each
+// 32, serially: 158 us instead of %JOIN% at 64 requests of 128 to 4096 tokens.)
 #pragma once
 
 #include "common.cuh"

@@ -95,7 +95,7 @@ _PROTOS = {
                               c_p, c_p], 1),
     "pse_tree_masks": ([c_p, c_p, c_i32, c_i32, c_i32, c_p, c_p, c_p], 1),
     "pse_token_tree_attention": ([BlockState, KVLayer, HeadView, HeadView, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_p,
-                                  c_i32, c_f32, c_p, c_sz, c_p], 1),
+                                  c_i32, c_f32, c_p, c_sz, c_p], 2),
     "pse_scatter_rows": ([c_p, c_i64, c_p, c_i32, c_i32, c_p, c_i64, c_i32, c_p], 1),
     "pse_attention_force_generic": ([c_i32], 0),
     "pse_accept_select": ([c_i32], 0),

@@ -75,25 +75,10 @@ def tree_masks(parents: torch.Tensor, counts) -> TokenTrees:
     return trees
 
 
-_workspaces: dict = {}
-
-
 def token_tree_workspace(head_dim: int, device) -> torch.Tensor:
-    """A workspace for ``token_tree_attention`` (its head zeroed).  Calls that
-    may overlap on the GPU need one each."""
-    return torch.zeros(N.size_call("pse_token_tree_workspace", head_dim), dtype=torch.uint8, device=device)
-
-
-def _workspace(head_dim: int, device) -> torch.Tensor:
-    """The current stream's own workspace.  A call under capture gets one of
-    its graph instead, so a replay never shares it with other work."""
-    if torch.cuda.is_current_stream_capturing():
-        return token_tree_workspace(head_dim, device)
-    key = (device, N.stream_ptr())
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < N.size_call("pse_token_tree_workspace", head_dim):
-        ws = _workspaces[key] = token_tree_workspace(head_dim, device)
-    return ws
+    """A workspace for ``token_tree_attention``, for callers that keep one (its
+    contents do not matter).  Calls that may overlap on the GPU need one each."""
+    return torch.empty(N.size_call("pse_token_tree_workspace", head_dim), dtype=torch.uint8, device=device)
 
 
 def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor, context: torch.Tensor,
@@ -122,7 +107,7 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     check_heads("out", out, hd, q, q.shape[1])
     if workspace is None:
-        workspace = _workspace(hd, q.device)
+        workspace = token_tree_workspace(hd, q.device)
     N.call("pse_token_tree_attention", cache.state, cache.layer(layer), head_view(q), head_view(out),
            slots.data_ptr(), context.data_ptr(), trees.offsets.data_ptr(), rows, trees.nodes, trees.max_nodes,
            trees.masks.data_ptr(), trees.words, 1.0 / math.sqrt(hd) if scale is None else float(scale),
