@@ -152,8 +152,16 @@ def load(require_cuda: bool = True):
     return _lib
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device.  (Torch's raw query where it
+    has one: building a Stream object costs more than a small launch.)"""
+    if _raw_stream is None or _current_device is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_current_device())
 
 
 def call(name: str, *args) -> None:
@@ -162,6 +170,17 @@ def call(name: str, *args) -> None:
     if rc != 0:
         raise RuntimeError(f"{name} failed with code {rc}")
     launches[name] += _PROTOS[name][1]
+
+
+def fn(name: str):
+    """The library's function of that name, for callers that keep it; they
+    raise for a non-zero code with ``failed`` and count in ``launches``."""
+    lib = _lib if _lib is not None else load()
+    return getattr(lib, name)
+
+
+def failed(name: str, rc: int) -> RuntimeError:
+    return RuntimeError(f"{name} failed with code {rc}")
 
 
 def size_call(name: str, *args) -> int:

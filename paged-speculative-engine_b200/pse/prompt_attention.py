@@ -10,7 +10,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from .rotary import check_heads, head_view
+from .rotary import head_view
 
 
 class PackedPrompts:
@@ -33,6 +33,9 @@ class PackedPrompts:
             raise ValueError(f"{self.tokens} packed tokens (at most 2^31 - 1)")
         self.q_heads, self.kv_heads = int(q_heads), int(kv_heads)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.index = self.device.index if self.device.index is not None else torch.cuda.current_device()
+        self.device = torch.device("cuda", self.index)
+        self.fn = N.fn("pse_prompt_attention")
         self.n_cta = torch.cuda.get_device_properties(self.device).multi_processor_count
         host = np.asarray(lens, dtype=np.int32)
         size = ctypes.c_int64(0)
@@ -44,6 +47,7 @@ class PackedPrompts:
         self.n_items = (size.value - (self.n_cta + 4) // 4 * 4) // 4
         self.plan = torch.from_numpy(plan).to(self.device)
         self.status = self.plan[size.value:size.value + 1]
+        self._plan_ptr, self._status_ptr = self.plan.data_ptr(), self.status.data_ptr()
 
     def offsets(self) -> list:
         """First token of each prompt, and the total."""
@@ -68,22 +72,21 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompts:
     the packing's total.  ``scale`` defaults to 1 / sqrt(head_dim).  Returns
     [T, q_heads, head_dim] (``out`` if given, which must not overlap the
     inputs)."""
-    if not torch.is_tensor(q) or q.dim() != 3:
-        raise ValueError("q must be a [tokens, heads, head_dim] tensor")
-    hd = q.shape[2]
+    shape, dtype, dev = getattr(q, "shape", ()), getattr(q, "dtype", None), prompts.index
+    hd = shape[2] if len(shape) == 3 else 0
     if not 0 < hd <= 256:
-        raise ValueError(f"head_dim must be 1 to 256, got {hd}")
-    check_heads("q", q, hd, heads=prompts.q_heads)
-    if q.shape[0] != prompts.tokens:
-        raise ValueError(f"{q.shape[0]} tokens, but the prompts hold {prompts.tokens}")
-    if q.device != prompts.device:
-        raise ValueError(f"the prompts are on {prompts.device}, q on {q.device}")
-    check_heads("k", k, hd, q, prompts.kv_heads)
-    check_heads("v", v, hd, q, prompts.kv_heads)
+        raise ValueError(f"q must be [tokens, heads, head_dim] with a head_dim of 1 to 256, got {tuple(shape)}")
+    T = prompts.tokens
+    qv = head_view("q", q, T, prompts.q_heads, hd, dtype, dev)
+    kv = head_view("k", k, T, prompts.kv_heads, hd, dtype, dev)
+    vv = head_view("v", v, T, prompts.kv_heads, hd, dtype, dev)
+    code = N.dtype_code(dtype)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    check_heads("out", out, hd, q, prompts.q_heads)
-    N.call("pse_prompt_attention", head_view(q), head_view(k), head_view(v), head_view(out), q.shape[0], hd,
-           N.dtype_code(q.dtype), 1.0 / math.sqrt(hd) if scale is None else float(scale), prompts.plan.data_ptr(),
-           prompts.n_cta, prompts.n_items, prompts.status.data_ptr(), N.stream_ptr())
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ov = head_view("out", out, T, prompts.q_heads, hd, dtype, dev)
+    rc = prompts.fn(qv, kv, vv, ov, T, hd, code, 1.0 / math.sqrt(hd) if scale is None else float(scale),
+                    prompts._plan_ptr, prompts.n_cta, prompts.n_items, prompts._status_ptr, N.stream_ptr())
+    if rc:
+        raise N.failed("pse_prompt_attention", rc)
+    N.launches["pse_prompt_attention"] += 1
     return out

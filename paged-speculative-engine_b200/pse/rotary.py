@@ -101,6 +101,9 @@ class RotaryPlan:
         f, self.factor = rotary_frequencies(rotary_dim, float(theta), scaling)
         self.head_dim, self.rotary_dim, self.interleaved = int(head_dim), rotary_dim, bool(interleaved)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.index = self.device.index if self.device.index is not None else torch.cuda.current_device()
+        self.device = torch.device("cuda", self.index)
+        self.fn, self.append_fn = N.fn("pse_rotary"), N.fn("pse_rotary_append")
         self.turns = torch.tensor([x / (2 * math.pi) for x in f], dtype=torch.float64, device=self.device)
         self.spec = N.RotarySpec(self.turns.data_ptr(), self.factor, self.head_dim, self.rotary_dim,
                                  int(self.interleaved))
@@ -109,38 +112,38 @@ class RotaryPlan:
 _NO_HEADS = N.HeadView(None, 0, 0, 0)
 
 
-def head_view(t: torch.Tensor) -> N.HeadView:
-    return N.HeadView(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1])
-
-
-def check_heads(name: str, t: torch.Tensor, head_dim: int, like: torch.Tensor | None = None,
-                heads: int | None = None) -> None:
-    """[tokens, heads, head_dim], the last axis contiguous, on a GPU; tokens,
-    dtype and device as ``like`` has them."""
-    if not torch.is_tensor(t) or t.dim() != 3 or t.shape[2] != head_dim:
-        raise ValueError(f"{name} must be a [tokens, heads, {head_dim}] tensor, got "
-                         f"{tuple(t.shape) if torch.is_tensor(t) else type(t).__name__}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be on a GPU")
-    N.dtype_code(t.dtype)
-    if t.stride(2) != 1 and t.numel():
+def head_view(name: str, t: torch.Tensor, tokens, heads, head_dim: int, dtype, device: int) -> N.HeadView:
+    """The library's view of ``t``, which must be [tokens, heads, head_dim] with
+    a contiguous last axis, of ``dtype``, on GPU ``device`` (tokens or heads
+    None: any)."""
+    try:
+        T, H, D = t.shape
+        s0, s1, s2 = t.stride()
+    except (AttributeError, ValueError, TypeError):
+        raise ValueError(f"{name} must be a [tokens, heads, {head_dim}] tensor") from None
+    if D != head_dim or (tokens is not None and T != tokens) or (heads is not None and H != heads):
+        raise ValueError(f"{name} must be [{'tokens' if tokens is None else tokens}, "
+                         f"{'heads' if heads is None else heads}, {head_dim}], got {tuple(t.shape)}")
+    if t.dtype is not dtype or t.get_device() != device:
+        raise ValueError(f"{name} must be {dtype} on GPU {device}, got {t.dtype} on {t.device}")
+    if s2 != 1 and T * H * D:
         raise ValueError(f"{name}'s last axis must be contiguous")
-    if heads is not None and t.shape[1] != heads:
-        raise ValueError(f"{name} must have {heads} heads, got {t.shape[1]}")
-    if like is not None and (t.shape[0] != like.shape[0] or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} must match q in tokens, dtype and device")
+    return N.HeadView(t.data_ptr(), s0, s1, H)
 
 
-def check_index(name: str, t: torch.Tensor, n: int, device) -> None:
-    if not torch.is_tensor(t) or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or \
-            not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on {device}")
+def index_ptr(name: str, t: torch.Tensor, n: int, device: int) -> int:
+    """The address of ``t``, a contiguous int32 tensor of n entries on GPU ``device``."""
+    if not torch.is_tensor(t) or t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or \
+            t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on GPU {device}")
+    return t.data_ptr()
 
 
-def _check_out(name: str, out: torch.Tensor, src: torch.Tensor, head_dim: int) -> None:
-    check_heads(name, out, head_dim, src, src.shape[1])
-    if out.data_ptr() == src.data_ptr() and out.stride() != src.stride() and src.numel():
+def _out_view(name: str, out: torch.Tensor, src: torch.Tensor, view: N.HeadView, head_dim: int, dtype, device: int):
+    v = head_view(name, out, src.shape[0], view.heads, head_dim, dtype, device)
+    if v.data == view.data and (v.tok_stride != view.tok_stride or v.head_stride != view.head_stride) and src.numel():
         raise ValueError(f"{name} overlaps its input with other strides")
+    return v
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, plan: RotaryPlan, *,
@@ -149,22 +152,23 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     the tokens' ``positions`` (int32 [T]); any token and head strides (views of
     a fused projection included).  Results go to ``q_out`` / ``k_out`` (which
     may be q / k themselves) or to new tensors, and are returned as (q, k)."""
-    check_heads("q", q, plan.head_dim)
-    check_index("positions", positions, q.shape[0], q.device)
-    if plan.device != q.device:
-        raise ValueError(f"the plan is on {plan.device}, q on {q.device}")
+    hd, dev, dtype = plan.head_dim, plan.index, getattr(q, "dtype", None)
+    qv = head_view("q", q, None, None, hd, dtype, dev)
+    code, T = N.dtype_code(dtype), q.shape[0]
+    pos = index_ptr("positions", positions, T, dev)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _check_out("q_out", q_out, q, plan.head_dim)
-    kv, kv_out = _NO_HEADS, _NO_HEADS
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
+    kv = ko = _NO_HEADS
     if k is not None:
-        check_heads("k", k, plan.head_dim, q)
+        kv = head_view("k", k, T, None, hd, dtype, dev)
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _check_out("k_out", k_out, k, plan.head_dim)
-        kv, kv_out = head_view(k), head_view(k_out)
-    N.call("pse_rotary", plan.spec, head_view(q), head_view(q_out), kv, kv_out, positions.data_ptr(), q.shape[0],
-           N.dtype_code(q.dtype), N.stream_ptr())
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        ko = _out_view("k_out", k_out, k, kv, hd, dtype, dev)
+    rc = plan.fn(plan.spec, qv, qo, kv, ko, pos, T, code, N.stream_ptr())
+    if rc:
+        raise N.failed("pse_rotary", rc)
+    N.launches["pse_rotary"] += 1
     return q_out, k_out
 
 
@@ -177,26 +181,25 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     that grew the rows).  ``positions`` are the rotary positions, which differ
     from the cache's for tree nodes.  ``k_out``, if given, receives the turned
     k as well.  Returns the turned q."""
-    check_heads("q", q, plan.head_dim)
-    check_heads("k", k, plan.head_dim, q, cache.n_heads)
-    check_heads("v", v, plan.head_dim, q, cache.n_heads)
-    if cache.head_dim != plan.head_dim or cache.dtype != q.dtype or cache.device != q.device:
-        raise ValueError("the cache must match q in head_dim, dtype and device")
-    if plan.device != q.device:
-        raise ValueError(f"the plan is on {plan.device}, q on {q.device}")
+    hd, dev, dtype = plan.head_dim, plan.index, cache.dtype
+    if cache.head_dim != hd or cache.device.index != dev:
+        raise ValueError("the cache and the plan must match in head_dim and device")
     if not 0 <= layer < cache.n_layers:
         raise ValueError(f"layer {layer} of a cache with {cache.n_layers}")
+    qv = head_view("q", q, None, None, hd, dtype, dev)
     T = q.shape[0]
-    for name, t in (("positions", positions), ("slots", slots), ("cache_positions", cache_positions)):
-        check_index(name, t, T, q.device)
+    kv = head_view("k", k, T, cache.n_heads, hd, dtype, dev)
+    vv = head_view("v", v, T, cache.n_heads, hd, dtype, dev)
+    pos = index_ptr("positions", positions, T, dev)
+    slot = index_ptr("slots", slots, T, dev)
+    at = index_ptr("cache_positions", cache_positions, T, dev)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _check_out("q_out", q_out, q, plan.head_dim)
-    kv_out = _NO_HEADS
-    if k_out is not None:
-        _check_out("k_out", k_out, k, plan.head_dim)
-        kv_out = head_view(k_out)
-    N.call("pse_rotary_append", cache.state, cache.layer(layer), plan.spec, head_view(q), head_view(q_out),
-           head_view(k), kv_out, head_view(v), positions.data_ptr(), slots.data_ptr(), cache_positions.data_ptr(), T,
-           N.stream_ptr())
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
+    ko = _NO_HEADS if k_out is None else _out_view("k_out", k_out, k, kv, hd, dtype, dev)
+    rc = plan.append_fn(cache.state, cache.layer(layer), plan.spec, qv, qo, kv, ko, vv, pos, slot, at, T,
+                        N.stream_ptr())
+    if rc:
+        raise N.failed("pse_rotary_append", rc)
+    N.launches["pse_rotary_append"] += 1
     return q_out

@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _native as N
-from .rotary import check_heads, check_index, head_view
+from .rotary import head_view, index_ptr
 
 MAX_NODES = 4096  # nodes of one request's tree
 
@@ -37,8 +37,10 @@ class TokenTrees:
         self.words = masks.shape[1]
         if self.max_nodes > 64 * self.words:
             raise ValueError(f"{self.words} mask words for a tree of {self.max_nodes} nodes")
-        self.masks, self.depths, self.device = masks, depths, masks.device
+        self.masks, self.depths, self.device, self.index = masks, depths, masks.device, masks.get_device()
         self.offsets = _offsets(self.counts, self.device) if offsets is None else offsets
+        self.fn = N.fn("pse_token_tree_attention")
+        self._masks_ptr, self._offsets_ptr = masks.data_ptr(), self.offsets.data_ptr()
 
     @classmethod
     def from_parents(cls, parents: torch.Tensor, counts) -> "TokenTrees":
@@ -64,7 +66,7 @@ def tree_masks(parents: torch.Tensor, counts) -> TokenTrees:
     n = sum(counts)
     if not torch.is_tensor(parents) or not parents.is_cuda:
         raise ValueError("parents must be on a GPU")
-    check_index("parents", parents, n, parents.device)
+    index_ptr("parents", parents, n, parents.get_device())
     words = max(1, (max(counts, default=0) + 63) // 64)
     offsets = _offsets(counts, parents.device)
     masks = torch.empty(n, words, dtype=torch.int64, device=parents.device)
@@ -75,10 +77,16 @@ def tree_masks(parents: torch.Tensor, counts) -> TokenTrees:
     return trees
 
 
+_workspace_sizes: dict = {}  # head_dim -> bytes
+
+
 def token_tree_workspace(head_dim: int, device) -> torch.Tensor:
     """A workspace for ``token_tree_attention``, for callers that keep one (its
     contents do not matter).  Calls that may overlap on the GPU need one each."""
-    return torch.empty(N.size_call("pse_token_tree_workspace", head_dim), dtype=torch.uint8, device=device)
+    size = _workspace_sizes.get(head_dim)
+    if size is None:
+        size = _workspace_sizes[head_dim] = N.size_call("pse_token_tree_workspace", head_dim)
+    return torch.empty(size, dtype=torch.uint8, device=device)
 
 
 def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor, context: torch.Tensor,
@@ -90,26 +98,25 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
     [rows] (``cache.slots_tensor``).  The nodes' K/V must be in the cache, node
     j at position context + j.  ``scale`` defaults to 1 / sqrt(head_dim).
     Returns [nodes, q_heads, head_dim]; a node that sees nothing gives zeros."""
-    hd = cache.head_dim
-    check_heads("q", q, hd)
-    if q.dtype != cache.dtype or q.device != cache.device or trees.device != q.device:
-        raise ValueError("q, the cache and the trees must match in dtype and device")
-    if q.shape[0] != trees.nodes:
-        raise ValueError(f"{q.shape[0]} queries, but the trees hold {trees.nodes} nodes")
-    if q.shape[1] == 0 or q.shape[1] % cache.n_heads or q.shape[1] // cache.n_heads > 64 or hd > 256:
-        raise ValueError(f"{q.shape[1]} query heads over {cache.n_heads} K/V heads of {hd}")
+    hd, dtype, dev = cache.head_dim, cache.dtype, trees.index
+    if cache.device.index != dev:
+        raise ValueError("the cache and the trees must be on one device")
     if not 0 <= layer < cache.n_layers:
         raise ValueError(f"layer {layer} of a cache with {cache.n_layers}")
-    rows = len(trees.counts)
-    check_index("slots", slots, rows, q.device)
-    check_index("context", context, rows, q.device)
+    qv = head_view("q", q, trees.nodes, None, hd, dtype, dev)
+    heads, rows = qv.heads, len(trees.counts)
+    if heads == 0 or heads % cache.n_heads or heads // cache.n_heads > 64 or hd > 256:
+        raise ValueError(f"{heads} query heads over {cache.n_heads} K/V heads of {hd}")
+    slot, ctx = index_ptr("slots", slots, rows, dev), index_ptr("context", context, rows, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    check_heads("out", out, hd, q, q.shape[1])
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ov = head_view("out", out, trees.nodes, heads, hd, dtype, dev)
     if workspace is None:
         workspace = token_tree_workspace(hd, q.device)
-    N.call("pse_token_tree_attention", cache.state, cache.layer(layer), head_view(q), head_view(out),
-           slots.data_ptr(), context.data_ptr(), trees.offsets.data_ptr(), rows, trees.nodes, trees.max_nodes,
-           trees.masks.data_ptr(), trees.words, 1.0 / math.sqrt(hd) if scale is None else float(scale),
-           workspace.data_ptr(), workspace.numel(), N.stream_ptr())
+    rc = trees.fn(cache.state, cache.layer(layer), qv, ov, slot, ctx, trees._offsets_ptr, rows, trees.nodes,
+                  trees.max_nodes, trees._masks_ptr, trees.words, 1.0 / math.sqrt(hd) if scale is None else float(scale),
+                  workspace.data_ptr(), workspace.numel(), N.stream_ptr())
+    if rc:
+        raise N.failed("pse_token_tree_attention", rc)
+    N.launches["pse_token_tree_attention"] += 2
     return out
