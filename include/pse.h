@@ -455,8 +455,8 @@ int pse_tree_masks(const int32_t *parents, const int32_t *node_off, int32_t rows
  * its mask (`words` 64-bit words per node; bits past the row's nodes are
  * ignored, and a node need not see itself).  A node that sees nothing gives
  * zero, as do the nodes of a row with an invalid slot or a context the block
- * table cannot hold.  max_nodes bounds the rows' node counts (it picks the
- * kernel's shape; max_nodes <= 64 words).  ctx, slots and node_off are read on
+ * table cannot hold.  max_nodes bounds the rows' node counts (max_nodes <= 64
+ * words; a row with more is left out, its output unwritten).  ctx, slots and node_off are read on
  * the device only, so the call can be captured and replayed with other values.
  * workspace: pse_token_tree_workspace() bytes, 16-byte aligned, written before
  * it is read (what stands in it does not matter); calls that share one must

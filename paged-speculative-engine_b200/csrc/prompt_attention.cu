@@ -131,8 +131,8 @@ int simt_attention(const Args& a, cudaStream_t s) {
 //   warps 0-3, 4-7  the softmax of stream 0 and 1, a thread per row
 //                   (attention_tile.cuh), and the item's output
 //   warp 8          TMA: K and V tiles through a ring of slots
-//   warp 9          one thread issues the products: S = Q K^T into tensor
-//                   memory, O += P V with P there (over S's columns), V MN-major
+//   warp 9          the products: S = Q K^T into tensor memory, O += P V with
+//                   P there (over S's columns), V MN-major
 //   warp 10         looks through V tiles that some row must not see in whole
 //   warp 11         TMA: Q tiles, so that the ring runs on into the next item
 // While a stream's softmax runs, the tensor cores work on the other stream.
@@ -290,78 +290,81 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     } else if (warp == 9) {
       // -------------------------------------------------------------- products
-      {
-        const uint32_t el = elect_one();
-        constexpr uint32_t idesc_s = instr_desc(128, 0), idesc_o = instr_desc(HD, 1);
-        constexpr uint32_t kVAtoms = HD == 128 ? (uint32_t)kHalfBytes : 1024u;
-        int c = 0;             // slots used by earlier tiles: K of tile j at c + 2 j, V at c + 2 j + 1
-        int np[2] = {0, 0};    // weights consumed per stream
-        int no[2] = {0, 0};    // items finished per stream
-        int nq = 0;
-        bool run = true;
-        auto slot_wait = [&](int x) { return mbar_wait_warp(&slot_full[x % NS], (x / NS) & 1, vabort); };
-        auto scores = [&](int s, int x) {
-          const uint32_t qa = su32(q_s + s * kTileBytes), kb = su32(ring + (x % NS) * kTileBytes);
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-            mma_ss(el, tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
-          }
-          mma_commit(el, &s_full[s]);
-        };
-        for (int e = e0; run && e < e1; ++e) {
-          const TcItem it = decode(a, e, tpt);
-          if (it.n_max == 0) continue;
-          if (!mbar_wait_warp(q_full, nq & 1, vabort) || !slot_wait(c)) break;
-          ++nq;
-          fence_after();
-          for (int s = 0; s < 2; ++s)
-            if (it.n[s] > 0) scores(s, c);
-          mma_commit(el, &slot_empty[c % NS]);
-          if (it.n_max == 1) mma_commit(el, q_empty);
-          for (int j = 0; run && j < it.n_max; ++j) {
-            const int kx = c + 2 * (j + 1), vx = c + 2 * j + 1;
-            bool v_here = false, k_here = false;
-            for (int s = 0; run && s < 2; ++s) {
-              if (j >= it.n[s]) continue;
-              if (!v_here) run = slot_wait(vx);
-              v_here = true;
-              if (run && j == 0 && no[s] > 0) run = mbar_wait_warp(&o_empty[s], (no[s] - 1) & 1, vabort);
-              const uint32_t vb = su32(ring + (vx % NS) * kTileBytes);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if (run) run = mbar_wait_warp(&p_half[2 * s + h], np[s] & 1, vabort);
-                if (!run) break;
-                fence_after();
-#pragma unroll
-                for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                  mma_ts(el, tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
-                         idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-              }
-              if (!run) break;
-              ++np[s];
-              if (j + 1 == it.n[s]) {
-                mma_commit(el, &o_full[s]);
-                ++no[s];
-              } else {
-                if (!k_here) run = slot_wait(kx);
-                k_here = true;
-                if (!run) break;
-                fence_after();
-                scores(s, kx);
-              }
-            }
-            if (!run) break;
-            mma_commit(el, &slot_empty[vx % NS]);
-            if (k_here) {
-              mma_commit(el, &slot_empty[kx % NS]);
-              if (j + 2 == it.n_max) mma_commit(el, q_empty);
-            }
-          }
-          c += 2 * it.n_max;
+      const uint32_t el = elect_one();
+      const uint32_t full0 = su32(slot_full), empty0 = su32(slot_empty), ring0 = su32(ring), q0 = su32(q_s);
+      const uint32_t part0 = su32(p_half);
+      int slot = 0;
+      uint32_t fill = 0;
+      uint32_t parts = 0, outs = 3;
+      uint32_t nq = 0;
+      bool run = true;
+      auto next_slot = [&](int& i, uint32_t& par) {
+        i = slot;
+        par = fill;
+        if (++slot == NS) {
+          slot = 0;
+          fill ^= 1;
         }
-        mma_commit(el, final_bar);
+      };
+      for (int e = e0; run && e < e1; ++e) {
+        const TcItem it = decode(a, e, tpt);
+        if (it.n_max == 0) continue;
+        const int n0 = it.n[0], n1 = it.n[1], n = it.n_max;
+        int k, v = 0;
+        uint32_t kp, vp = 0;
+        next_slot(k, kp);
+        run = mbar_wait3_warp(su32(q_full), nq, full0 + 8 * k, kp, full0 + 8 * k, kp, vabort);
+        nq ^= 1;
+        if (!run) break;
+        fence_after();
+        issue_scores<HD>(el, tmem + kColS, q0, ring0 + k * kTileBytes);
+        mma_commit(el, &s_full[0]);
+        if (n1 > 0) {
+          issue_scores<HD>(el, tmem + kColS + 128, q0 + kTileBytes, ring0 + k * kTileBytes);
+          mma_commit(el, &s_full[1]);
+        }
+        mma_commit(el, &slot_empty[k]);
+        if (n == 1) mma_commit(el, q_empty);
+#pragma unroll 1
+        for (int j = 0; run && j < n; ++j) {
+          next_slot(v, vp);
+          const bool more = j + 1 < n;
+          if (more) next_slot(k, kp);
+          const uint32_t vbar = full0 + 8 * v, kbar = more ? full0 + 8 * k : vbar;
+          if (!more) kp = vp;
+          bool here = false;  // the tile's V and the next K have been awaited
+          auto stream = [&](int s, int ns) {
+            if (j >= ns || !run) return;
+            const uint32_t s_col = tmem + kColS + s * 128, o_col = tmem + kColO + s * 128, part = part0 + 16 * s;
+            const uint32_t np = parts >> s & 1u;
+            if (j == 0) run = mbar_wait_warp(&o_empty[s], outs >> s & 1u, vabort);
+            run = run && (here ? mbar_wait_warp(part, np, vabort) : mbar_wait3_warp(part, np, vbar, vp, kbar, kp, vabort));
+            here = true;
+            if (!run) return;
+            fence_after();
+            issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 0, j == 0);
+            run = mbar_wait_warp(part + 8, np, vabort);
+            if (!run) return;
+            fence_after();
+            issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 1, false);
+            parts ^= 1u << s;
+            if (j + 1 == ns) {
+              mma_commit(el, &o_full[s]);
+              outs ^= 1u << s;
+            } else {
+              issue_scores<HD>(el, s_col, q0 + s * kTileBytes, ring0 + k * kTileBytes);
+              mma_commit(el, &s_full[s]);
+            }
+          };
+          stream(0, n0);
+          stream(1, n1);
+          if (!run) break;
+          mma_commit(el, &slot_empty[v]);
+          if (more) mma_commit(el, &slot_empty[k]);
+          if (j + 2 == n) mma_commit(el, q_empty);
+        }
       }
+      mma_commit(el, final_bar);
     } else if (warp == 10) {
       // -------------------------------------------------------------- guard
       int c = 0, g = 0, items = 0;
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float inv = row.l == 0.f ? 0.f : 1.f / row.l;
       __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + (int64_t)(it.tok0 + tok) * a.o_tok +
                            (int64_t)(it.hk * a.group + rg) * a.o_head;
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < HD / 32; ++h) {
         uint32_t u[32];
         float* o = reinterpret_cast<float*>(u);

@@ -14,7 +14,7 @@
 namespace pse {
 namespace t5 {
 
-constexpr uint32_t kSpinLimit = 1u << 22;
+constexpr uint32_t kSpinLimit = 1u << 18;  // tries, a few microseconds each
 
 __device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -22,8 +22,14 @@ __device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvt
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(bar)), "r"(count) : "memory");
 }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(bar)) : "memory");
@@ -37,13 +43,15 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait that also gives up once another role of the CTA has.
+// Bounded wait that also gives up once another role of the CTA has.  (Each try
+// suspends the thread in hardware for a while.  The loop is this short because
+// it stands in some thirty places: kernels whose warps walk different code
+// spend their time fetching it when it outgrows the instruction cache.)
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
   for (uint32_t n = 0; n < kSpinLimit; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((n & 15) == 15 && *abort_flag) return false;
-    if (n >= 64) __nanosleep(32);
+    if (*abort_flag) return false;
   }
   *abort_flag = 1;
   return false;
@@ -61,6 +69,25 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 }
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return mbar_wait_warp(su32(bar), parity, abort_flag);
+}
+// Waits for three barriers at once (repeat one for fewer): their polls are on
+// their way together.
+__device__ __forceinline__ bool mbar_wait3_warp(uint32_t a, uint32_t pa, uint32_t b, uint32_t pb, uint32_t c, uint32_t pc,
+                                                volatile int* abort_flag) {
+  bool ok = false;
+#pragma unroll 1
+  for (uint32_t n = 0; n < kSpinLimit; ++n) {
+    const bool x = mbar_try_wait(a, pa), y = mbar_try_wait(b, pb), z = mbar_try_wait(c, pc);
+    if (x && y && z) {
+      ok = true;
+      break;
+    }
+    if (*abort_flag) break;
+  }
+  if (!ok) *abort_flag = 1;
+  ok = __all_sync(0xffffffffu, ok);
+  __syncwarp();
+  return ok;
 }
 // Bounded wait of the exit path (no abort check).
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
@@ -82,6 +109,17 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(su32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(su32(bar))
+      : "memory");
+}
+
+// The same from a converged warp, issued by its elected lane (see mma_ss below).
+__device__ __forceinline__ void tma_load_2d(uint32_t elected, uint32_t dst, const CUtensorMap* map, int x, int y,
+                                            uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %5, 0;\n"
+      " @e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];\n}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(elected)
       : "memory");
 }
 
@@ -137,6 +175,28 @@ __device__ __forceinline__ void mma_commit(uint32_t elected, uint64_t* bar) {
       " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(su32(bar)),
       "r"(elected)
       : "memory");
+}
+
+// S = Q K^T (M = N = 128) over head_dim HD: both operands as HD / 64 column
+// halves of 16 KB.
+template <int HD>
+__device__ __forceinline__ void issue_scores(uint32_t elected, uint32_t d, uint32_t q, uint32_t k) {
+  const uint64_t a = desc_kmajor(q), b = desc_kmajor(k);
+#pragma unroll
+  for (int kk = 0; kk < HD / 16; ++kk) {
+    const uint64_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+    mma_ss(elected, d, a + off, b + off, instr_desc(128, 0), kk > 0);
+  }
+}
+// O += P V for keys 64 h .. 64 h + 63 of a tile (N = HD), P in tensor memory, V
+// MN-major; fresh: the first product overwrites O.
+template <int HD>
+__device__ __forceinline__ void issue_values(uint32_t elected, uint32_t o, uint32_t p, uint32_t v, int h, bool fresh) {
+  const uint64_t b = desc_mnmajor(v + h * 8192, HD == 128 ? 128u * 128u : 1024u);
+  p += 32 * h;
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk)
+    mma_ts(elected, o, p + 8 * kk, b + ((kk * 2048) >> 4), instr_desc(HD, 1), kk > 0 || !fresh);
 }
 
 #define PSE_T5_R32(r)                                                                                               \

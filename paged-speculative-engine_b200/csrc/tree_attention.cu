@@ -122,7 +122,7 @@ int launch_join(const Args& a, int ctas, int max_nodes, int tile_rows, int tile_
 template <typename T, int RPT, int NC>
 __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a) {
   extern __shared__ float smem[];
-  __shared__ long long tmp[40];
+  __shared__ int tmp[36];
   constexpr int BQ = 16 * RPT, TILE = simt::BK;
   const Span span = my_span<TILE>(a.rows, a.block_nodes, tmp);
   Cut cut{-1, 0, 0, 0};
@@ -172,8 +172,9 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
       __syncthreads();
       t.step(k0 + TILE > g.r.ctx || g.r.slot < 0, [&](int r, int key) {
         if (r >= nr || k0 + key >= keys) return false;
-        const int64_t* m = a.masks + (int64_t)(g.r.n0 + node0 + r / group) * a.words;
-        return (visible32(m, a.words, g.r, k0 + (key & ~31)) >> (key & 31) & 1u) != 0u;
+        const uint32_t* m = reinterpret_cast<const uint32_t*>(a.masks + (int64_t)(g.r.n0 + node0 + r / group) * a.words);
+        const auto word = [&](int i) { return __ldg(m + i); };
+        return (visible32(word, a.words, g.r, k0 + (key & ~31)) >> (key & 31) & 1u) != 0u;
       });
     }
     T* out = reinterpret_cast<T*>(a.out);
@@ -240,6 +241,7 @@ int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
   const int rpt = simt_rows(max_nodes * a.rows.group);
   a.block_nodes = 16 * rpt / a.rows.group;
   a.part_rows = 16 * rpt;
+  if (!countable(a.rows, simt::BK, a.block_nodes)) return PSE_EINVAL;
   const int rc = rpt == 1 ? simt_nc<T, 1>(a, kMaxCtas, s) : simt_nc<T, 4>(a, kMaxCtas, s);
   return rc == PSE_OK ? launch_join<T>(a, kMaxCtas, max_nodes, a.part_rows, a.part_rows, s) : rc;
 }
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int kTileBytes = 128 * HD * 2, kHalves = HD / 64;
   constexpr int HDS = NQ == 1 ? HD / 2 : HD;  // output columns of a softmax thread
   extern __shared__ uint8_t smem_raw[];
-  __shared__ long long span_tmp[40];
+  __shared__ int span_tmp[36];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                     // [NQ][128 x HD]
   uint8_t* ring = q_s + NQ * kTileBytes;   // [NS][128 x HD]
@@ -355,17 +357,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   };
   // tiles from here on hold keys that some node may not see
   auto guard_from = [&](const Segment& x) { return max(x.t0, x.r.slot < 0 ? 0 : x.r.ctx >> 7); };
-  // ring positions of a segment's K and V tiles i of nt, in the order they are
-  // needed: the streams of NQ = 1 start on K tiles 0 and 1
-  auto k_at = [](int i) { return NQ == 1 ? max(2 * i - 1, 0) : 2 * i; };
-  auto v_at = [](int i, int nt) { return NQ == 1 && i < nt - 1 ? 2 * i + 2 : 2 * i + 1; };
+  // ring positions of a segment's K and V tiles i
+  auto k_at = [](int i) { return 2 * i; };
+  auto v_at = [](int i) { return 2 * i + 1; };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 8) {
       // -------------------------------------------------------------- pages
       const int bs = a.block_size, ppt = 128 / bs, oob = a.num_blocks * a.rows.kv_heads * bs;
-      int c = 0, gd = 0;
+      const uint32_t el = elect_one();
+      const uint32_t empty0 = su32(slot_empty), full0 = su32(slot_full), guard0 = su32(guard_full), ring0 = su32(ring);
+      int gd = 0, slot = 0;
+      uint32_t fill = 0;
       bool run = true;
       while (run && walk.next(g)) {
         const int nt = g.t1 - g.t0, g0 = guard_from(g);
@@ -379,55 +383,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int b = __ldg(table + pi);
           return b >= 0 && b < a.num_blocks ? (b * a.rows.kv_heads + g.hk) * bs : oob;
         };
-        int chunk_rows[2] = {page(lane), page(32 + lane)};
+        int cur = page(lane), nxt = page(32 + lane);
         const int tpc = 32 / ppt;  // tiles per chunk
-        int chunk = 0;             // chunk held in chunk_rows[0]; [1] is the next one
-        for (int x = 0; run && x < 2 * nt; ++x) {
-          bool is_v;
-          int i;
-          if (NQ == 1) {
-            // K0 K1 V0 K2 V1 K3 ... V(nt-2) V(nt-1)
-            if (x == 0) {
-              is_v = false;
-              i = 0;
-            } else if (x == 2 * nt - 1) {
-              is_v = true;
-              i = nt - 1;
-            } else {
-              is_v = (x & 1) == 0;
-              i = is_v ? (x - 2) >> 1 : (x + 1) >> 1;
-            }
-          } else {
-            is_v = x & 1;
-            i = x >> 1;
+        for (int i = 0; run && i < nt; ++i) {
+          const int src = (i % tpc) * ppt;
+          if (i > 0 && src == 0) {
+            cur = nxt;
+            nxt = page(32 * (i / tpc + 1) + lane);
           }
-          // V runs at most two tiles behind K: its tile is in the chunk held or the next
-          if (i / tpc > chunk && is_v) {
-            ++chunk;
-            chunk_rows[0] = chunk_rows[1];
-            chunk_rows[1] = page(32 * (chunk + 1) + lane);
-          }
-          const int src = (i % tpc) * ppt + (lane & (ppt - 1));
-          const int lo = __shfl_sync(0xffffffffu, chunk_rows[0], src), hi = __shfl_sync(0xffffffffu, chunk_rows[1], src);
-          const int y = i / tpc == chunk ? lo : hi;
-          const int s = c % NS;
-          run = mbar_wait_warp(&slot_empty[s], ((c / NS) & 1) ^ 1, vabort);
-          if (!run) break;
-          const bool guarded = is_v && g.t0 + i >= g0;
-          uint64_t* bar = guarded ? &guard_full[gd % kGuards] : &slot_full[s];
-          if (lane == 0) {
-            last_bar[s] = guarded ? (NS + gd % kGuards) * 2 + ((gd / kGuards) & 1) : s * 2 + ((c / NS) & 1);
-            mbar_expect_tx(bar, kTileBytes);
-          }
-          __syncwarp();
-          if (lane < ppt) {
+          // the tile's K, then its V, page by page with operands uniform over the warp
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-              tma_load_2d(ring + s * kTileBytes + h * kHalfBytes + lane * bs * 128, is_v ? &tmv : &tmk, h * 64, y, bar);
+          for (int kv = 0; kv < 2; ++kv) {
+            run = run && mbar_wait_warp(empty0 + 8 * slot, fill ^ 1, vabort);
+            if (!run) break;
+            const bool guarded = kv == 1 && g.t0 + i >= g0;
+            const uint32_t bar = guarded ? guard0 + 8 * (gd % kGuards) : full0 + 8 * slot;
+            if (el) {
+              last_bar[slot] = guarded ? (NS + gd % kGuards) * 2 + ((gd / kGuards) & 1) : slot * 2 + (int)fill;
+              mbar_expect_tx(bar, kTileBytes);
+            }
+            uint32_t dst = ring0 + slot * kTileBytes;
+            for (int p = 0; p < ppt; ++p, dst += bs * 128) {
+              const int y = __shfl_sync(0xffffffffu, cur, src + p);
+#pragma unroll
+              for (int h = 0; h < kHalves; ++h) tma_load_2d(el, dst + h * kHalfBytes, kv ? &tmv : &tmk, h * 64, y, bar);
+            }
+            if (guarded) ++gd;
+            if (++slot == NS) {
+              slot = 0;
+              fill ^= 1;
+            }
           }
-          __syncwarp();
-          ++c;
-          if (guarded) ++gd;
         }
       }
     } else if (warp == 11) {
@@ -451,113 +437,123 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     } else if (warp == 9) {
       // -------------------------------------------------------------- products
-      {
-        const uint32_t el = elect_one();
-        constexpr uint32_t idesc_s = instr_desc(128, 0), idesc_o = instr_desc(HD, 1);
-        constexpr uint32_t kVAtoms = HD == 128 ? (uint32_t)kHalfBytes : 1024u;
-        int c = 0, np[2] = {0, 0}, no[2] = {0, 0}, nq = 0;
-        bool run = true;
-        auto slot_wait = [&](int x) { return mbar_wait_warp(&slot_full[x % NS], (x / NS) & 1, vabort); };
-        auto scores = [&](int s, int x) {
-          const uint32_t qa = su32(q_s + (NQ == 1 ? 0 : s) * kTileBytes), kb = su32(ring + (x % NS) * kTileBytes);
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-            mma_ss(el, tmem + kColS + s * 128, desc_kmajor(qa + off), desc_kmajor(kb + off), idesc_s, kk > 0);
+      const uint32_t el = elect_one();
+      const uint32_t full0 = su32(slot_full), ring0 = su32(ring), q0 = su32(q_s), part0 = su32(p_half);
+      int slot = 0;                  // next slot of the ring, and the parity of its fill
+      uint32_t fill = 0;
+      uint32_t parts = 0, outs = 3;  // per stream (bit): parity of its next weights, of its last output's reading
+      uint32_t nq = 0;
+      bool run = true;
+      auto next_slot = [&](int& i, uint32_t& par) {
+        i = slot;
+        par = fill;
+        if (++slot == NS) {
+          slot = 0;
+          fill ^= 1;
+        }
+      };
+      auto scores = [&](int s, int k) {
+        fence_after();
+        issue_scores<HD>(el, tmem + kColS + s * 128, q0 + (NQ == 1 ? 0 : s) * kTileBytes, ring0 + k * kTileBytes);
+        mma_commit(el, &s_full[s]);
+      };
+      // O_s += P_s V with the V of slot v; the first wait takes two tiles with it
+      auto values = [&](int s, int v, bool fresh, uint32_t bar1, uint32_t par1, uint32_t bar2, uint32_t par2) {
+        const uint32_t s_col = tmem + kColS + s * 128, o_col = tmem + kColO + s * 128, part = part0 + 16 * s;
+        const uint32_t par = parts >> s & 1u, vb = ring0 + v * kTileBytes;
+        run = run && mbar_wait3_warp(part, par, bar1, par1, bar2, par2, vabort);
+        if (!run) return;
+        fence_after();
+        issue_values<HD>(el, o_col, s_col, vb, 0, fresh);
+        run = mbar_wait_warp(part + 8, par, vabort);
+        if (!run) return;
+        fence_after();
+        issue_values<HD>(el, o_col, s_col, vb, 1, false);
+        parts ^= 1u << s;
+      };
+      while (run && walk.next(g)) {
+        int n[2];
+        counts(g, n);
+        const int nt = g.t1 - g.t0;
+        int k, v, ahead = 0;
+        uint32_t kp, vp, ap = 0;
+        next_slot(k, kp);
+        run = mbar_wait3_warp(su32(q_full), nq, full0 + 8 * k, kp, full0 + 8 * k, kp, vabort);
+        nq ^= 1;
+        if (!run) break;
+        scores(0, k);
+        if (NQ == 1) {
+          // tiles i and i + 1 are on the streams' way; ring order K0 V0 K1 V1 ...
+          mma_commit(el, &slot_empty[k]);
+          next_slot(v, vp);
+          int v1 = v;
+          uint32_t v1p = vp;
+          if (nt > 1) {
+            next_slot(k, kp);
+            run = mbar_wait_warp(full0 + 8 * k, kp, vabort);
+            if (!run) break;
+            scores(1, k);
+            mma_commit(el, &slot_empty[k]);
+            next_slot(v1, v1p);
           }
-          mma_commit(el, &s_full[s]);
-        };
-        // O_s += P_s V once the weights stand there
-        auto values = [&](int s, int x, bool first) -> bool {
-          const uint32_t vb = su32(ring + (x % NS) * kTileBytes);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!mbar_wait_warp(&p_half[2 * s + h], np[s] & 1, vabort)) return false;
-            fence_after();
-#pragma unroll
-            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-              mma_ts(el, tmem + kColO + s * 128, tmem + kColS + s * 128 + kk * 8, desc_mnmajor(vb + kk * 2048, kVAtoms),
-                     idesc_o, (!first || kk > 0) ? 1u : 0u);
-          }
-          ++np[s];
-          return true;
-        };
-        while (run && walk.next(g)) {
-          int n[2];
-          counts(g, n);
-          const int nt = g.t1 - g.t0;
-          if (!mbar_wait_warp(q_full, nq & 1, vabort)) break;
-          ++nq;
-          if (NQ == 1) {
-            for (int i = 0; run && i < min(nt, 2); ++i) {
-              run = slot_wait(c + k_at(i));
-              if (!run) break;
-              fence_after();
-              scores(i, c + k_at(i));
-              mma_commit(el, &slot_empty[(c + k_at(i)) % NS]);
+          if (nt <= 2) mma_commit(el, q_empty);
+          // both outputs of the segment before have been read
+          run = mbar_wait_warp(&o_empty[0], outs & 1u, vabort);
+#pragma unroll 1
+          for (int i = 0; run && i < nt; ++i) {
+            const int s = i & 1;
+            const bool more = i + 2 < nt;
+            const uint32_t vbar = full0 + 8 * v;
+            if (more) {
+              next_slot(ahead, ap);
             }
-            if (run && nt <= 2) mma_commit(el, q_empty);
-            for (int i = 0; run && i < nt; ++i) {
-              const int s = i & 1, vx = c + v_at(i, nt);
-              run = slot_wait(vx);
-              // both outputs of the segment before have been read
-              if (run && i == 0 && no[0] > 0) run = mbar_wait_warp(&o_empty[0], (no[0] - 1) & 1, vabort);
-              if (!run || !values(s, vx, i < 2)) {
-                run = false;
-                break;
-              }
-              mma_commit(el, &slot_empty[vx % NS]);
-              if (i + 2 < nt) {
-                const int kx = c + k_at(i + 2);
-                run = slot_wait(kx);
-                if (!run) break;
-                fence_after();
-                scores(s, kx);
-                mma_commit(el, &slot_empty[kx % NS]);
-                if (i + 3 == nt) mma_commit(el, q_empty);
+            values(s, v, i < 2, vbar, vp, more ? full0 + 8 * ahead : vbar, more ? ap : vp);
+            if (!run) break;
+            mma_commit(el, &slot_empty[v]);
+            v = v1;
+            vp = v1p;
+            if (more) {
+              scores(s, ahead);
+              mma_commit(el, &slot_empty[ahead]);
+              if (i + 3 == nt) mma_commit(el, q_empty);
+              next_slot(v1, v1p);
+            } else {
+              mma_commit(el, &o_full[s]);
+            }
+          }
+          outs ^= 1u;
+        } else {
+          if (n[1] > 0) scores(1, k);
+          mma_commit(el, &slot_empty[k]);
+          if (nt == 1) mma_commit(el, q_empty);
+#pragma unroll 1
+          for (int i = 0; run && i < nt; ++i) {
+            next_slot(v, vp);
+            const bool more = i + 1 < nt;
+            if (more) next_slot(k, kp);
+            const uint32_t vbar = full0 + 8 * v, kbar = more ? full0 + 8 * k : vbar;
+            if (!more) kp = vp;
+            auto stream = [&](int s) {
+              if (i == 0) run = run && mbar_wait_warp(&o_empty[s], outs >> s & 1u, vabort);
+              values(s, v, i == 0, vbar, vp, kbar, kp);
+              if (!run) return;
+              if (more) {
+                scores(s, k);
               } else {
                 mma_commit(el, &o_full[s]);
+                outs ^= 1u << s;
               }
-            }
-            ++no[0];
-          } else {
-            run = slot_wait(c);
+            };
+            stream(0);
+            if (run && n[1] > 0) stream(1);
             if (!run) break;
-            fence_after();
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-              if (n[s] > 0) scores(s, c);
-            mma_commit(el, &slot_empty[c % NS]);
-            if (nt == 1) mma_commit(el, q_empty);
-            for (int i = 0; run && i < nt; ++i) {
-              const int vx = c + v_at(i, nt), kx = c + k_at(i + 1);
-              run = slot_wait(vx) && (i + 1 == nt || slot_wait(kx));
-  #pragma unroll
-            for (int s = 0; run && s < 2; ++s) {
-                if (n[s] == 0) continue;
-                if (i == 0 && no[s] > 0) run = mbar_wait_warp(&o_empty[s], (no[s] - 1) & 1, vabort);
-                if (!run || !values(s, vx, i == 0)) {
-                  run = false;
-                  break;
-                }
-                if (i + 1 == nt) {
-                  mma_commit(el, &o_full[s]);
-                  ++no[s];
-                } else {
-                  fence_after();
-                  scores(s, kx);
-                }
-              }
-              if (!run) break;
-              mma_commit(el, &slot_empty[vx % NS]);
-              if (i + 1 < nt) mma_commit(el, &slot_empty[kx % NS]);
-              if (i + 2 == nt) mma_commit(el, q_empty);
-            }
+            mma_commit(el, &slot_empty[v]);
+            if (more) mma_commit(el, &slot_empty[k]);
+            if (i + 2 == nt) mma_commit(el, q_empty);
           }
-          c += 2 * nt;
         }
-        mma_commit(el, final_bar);
       }
+      mma_commit(el, final_bar);
     } else {
       // -------------------------------------------------------------- guard
       int c = 0, gd = 0, items = 0;
@@ -570,7 +566,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             run = false;
             break;
           }
-          const int s = (c + v_at(t - g.t0, nt)) % NS;
+          const int s = (c + v_at(t - g.t0)) % NS;
           if (tile::clear_nonfinite(reinterpret_cast<uint4*>(ring + s * kTileBytes), kTileBytes / 16))
             marks |= 1 << min(t - g0, 31);
           if (lane == 0) {
@@ -587,7 +583,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int s = warp >> 2, q4 = warp & 3, r = tid & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16);
-    const int rt = r / group;
+    const int rt = r / group, rg = r - rt * group;
     int nt_done = 0, items = 0, no[2] = {0, 0};
     Cut cut{-1, 0, 0, 0};
     bool run = true;
@@ -600,8 +596,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool valid = rt < tpt && node < g.r.nodes;
       const uint32_t valid_rows = __ballot_sync(0xffffffffu, valid);
       const int g0 = guard_from(g);
-      const int64_t* mask = a.masks + (int64_t)(g.r.n0 + (valid ? node : 0)) * a.words;
-      auto bits = [&](int key0) { return visible32(mask, a.words, g.r, key0); };
+      const uint32_t* mask = reinterpret_cast<const uint32_t*>(a.masks + (int64_t)(g.r.n0 + (valid ? node : 0)) * a.words);
+      // the first word of the mask (all of it, up to 64 nodes) on its way early
+      const uint2 head = __ldg(reinterpret_cast<const uint2*>(mask));
+      auto bits = [&](int key0) {
+        return visible32([&](int i) { return i == 0 ? head.x : i == 1 ? head.y : __ldg(mask + i); }, a.words, g.r, key0);
+      };
       tile::RowState row;
       row.reset();
       for (int j = 0; j < n[s]; ++j, ++nt_done) {
@@ -635,7 +635,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         *reinterpret_cast<float2*>(x + s * 256 + 2 * r) = make_float2(row.m, row.l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&x_bar[q4]);
-        if (!mbar_wait_warp(&x_bar[q4], item & 1, vabort)) break;
+        const uint32_t full0 = su32(&o_full[0]);
+        run = mbar_wait3_warp(su32(&x_bar[q4]), item & 1, full0, no[0] & 1, n[1] > 0 ? full0 + 8 : full0,
+                              (n[1] > 0 ? no[1] : no[0]) & 1, vabort);
+        ++no[0];
+        no[1] += n[1] > 0 ? 1 : 0;
+        if (!run) break;
         const float2 s0 = *reinterpret_cast<const float2*>(x + 2 * r);
         const float2 s1 = *reinterpret_cast<const float2*>(x + 256 + 2 * r);
         M = fmaxf(s0.x, s1.x);
@@ -643,32 +648,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         f0 = ex2(s0.x - ms);
         f1 = n[1] > 0 ? ex2(s1.x - ms) : 0.f;
         L = s0.y * f0 + s1.y * f1;  // a sum is finite or the NaN of a score
+      } else {
+        run = mbar_wait_warp(&o_full[s], no[0] & 1, vabort);
+        ++no[0];
+        if (!run) break;
       }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if ((NQ == 1 || x == s) && n[x] > 0) {
-          if (run) run = mbar_wait_warp(&o_full[x], no[x] & 1, vabort);
-          ++no[x];
-        }
-      }
-      if (!run) break;
       fence_after();
       const int marks = g0 < g.t1 ? poison[item % kGuards] : 0;
       const bool whole = g.t0 == 0 && g.t1 == g.tiles;
       const float inv = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
-      auto out_of = [&](int row_in_tile) {
-        const int t = row_in_tile / group;
-        return reinterpret_cast<__nv_bfloat16*>(a.out) +
-               (int64_t)(g.r.n0 + g.block * a.block_nodes + (NQ == 2 ? s * tpt : 0) + t) * a.o_tok +
-               (int64_t)(g.hk * group + row_in_tile - t * group) * a.o_head + (NQ == 1 ? s * HDS : 0);
-      };
       float* mine = part(a, blockIdx.x, g.t0 == 0);
       const int prow = (NQ == 2 ? s * 128 : 0) + r;
       if (g.t0 == 0 && !whole)
         cut = Cut{owner(span, g.first + g.tiles - 1), g.r.n0 + g.block * a.block_nodes,
                   min(a.block_nodes, g.r.nodes - g.block * a.block_nodes), g.hk};
-      __nv_bfloat16* dst = out_of(r);
-#pragma unroll
+      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + (int64_t)(g.r.n0 + node) * a.o_tok +
+                           (int64_t)(g.hk * group + rg) * a.o_head + (NQ == 1 ? s * HDS : 0);
+#pragma unroll 1
       for (int h = 0; h < HDS / 32; ++h) {
         const int col = (NQ == 1 ? s * HDS : 0) + 32 * h;
         uint32_t u[32];
@@ -781,6 +777,7 @@ int launch_tc(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
   if (rc == 0) rc = g_pool_maps.get(a.v_pool, HD, pool_rows, HD * 2, 64u, a.block_size, PSE_EINVAL, &mv);
   if (rc) return rc;
   a.part_rows = 128 * NQ;
+  if (!countable(a.rows, 128, a.block_nodes)) return PSE_EINVAL;
   const cudaError_t e = launch_pdl(kern, dim3(kNumSMs), dim3(kTcThreads), smem, s, mq, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
   return launch_join<__nv_bfloat16>(a, kNumSMs, max_nodes, tpt * a.rows.group, 128, s);
@@ -861,6 +858,7 @@ extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse
   a.rows.rows = rows;
   a.rows.num_slots = st.num_slots;
   a.rows.n_nodes = n_nodes;
+  a.rows.max_nodes = max_nodes;
   a.rows.kv_heads = kv.kv_heads;
   a.rows.group = q.heads / kv.kv_heads;
   a.rows.max_keys = (int64_t)st.max_blocks * st.block_size;

@@ -22,7 +22,7 @@ struct Rows {
   const int32_t* slots;
   const int32_t* ctx;
   const int32_t* node_off;  // [rows + 1]
-  int rows, num_slots, n_nodes, kv_heads, group;
+  int rows, num_slots, n_nodes, max_nodes, kv_heads, group;
   int64_t max_keys;  // keys a block table can hold
 };
 
@@ -36,7 +36,7 @@ __device__ __forceinline__ Row read_row(const Rows& a, int i) {
   r.ctx = a.ctx[i];
   r.n0 = a.node_off[i];
   r.nodes = a.node_off[i + 1] - r.n0;
-  if (r.n0 < 0 || r.nodes < 0 || (int64_t)r.n0 + r.nodes > a.n_nodes) r.nodes = 0;
+  if (r.n0 < 0 || r.nodes < 0 || r.nodes > a.max_nodes || (int64_t)r.n0 + r.nodes > a.n_nodes) r.nodes = 0;
   if (r.slot < 0 || r.slot >= a.num_slots) r.slot = -1;
   // a context the table cannot hold is not one: its nodes see nothing
   if (r.ctx < 0 || (int64_t)r.ctx + r.nodes > a.max_keys) {
@@ -56,60 +56,56 @@ __device__ __forceinline__ int key_tiles(const Row& r) {
   return r.nodes > 0 ? (r.ctx + r.nodes + TILE - 1) / TILE : 0;
 }
 
+// All counts of tiles fit 31 bits (the entry point checks the largest that the
+// block table allows): 64-bit divisions took longer than the loads of a tile.
 struct Span {
-  long long begin, end, total;  // this CTA's tiles, all tiles
-  int ctas;                     // CTAs that have tiles
-  int row;                      // row of the first tile
-  long long off;                // its offset within the row
+  int begin, end;    // this CTA's tiles
+  int per, extra;    // tiles per CTA; the first `extra` CTAs have one more
+  int ctas;          // CTAs that have tiles
+  int row, off;      // row of the first tile, and its offset within the row
 };
 
-// All threads of the CTA; `tmp` holds 40 long longs of shared memory.
 template <int TILE>
-__device__ Span my_span(const Rows& a, int block_nodes, long long* tmp) {
+__device__ __forceinline__ int row_weight(const Rows& a, const Row& r, int block_nodes) {
+  return r.nodes > 0 ? key_tiles<TILE>(r) * q_blocks(a, r, block_nodes) * a.kv_heads : 0;
+}
+
+// All threads of the CTA; `tmp` holds 36 ints of shared memory.
+template <int TILE>
+__device__ Span my_span(const Rows& a, int block_nodes, int* tmp) {
   const int per = (a.rows + blockDim.x - 1) / blockDim.x;
   const int lo = min(a.rows, (int)threadIdx.x * per), hi = min(a.rows, lo + per);
-  auto weight = [&](int i) -> long long {
-    const Row r = read_row(a, i);
-    return (long long)key_tiles<TILE>(r) * q_blocks(a, r, block_nodes) * a.kv_heads;
-  };
-  long long mine = 0, first = 0;
+  int mine = 0, first = 0;
   for (int i = lo; i < hi; ++i) {
-    const long long w = weight(i);
+    const int w = row_weight<TILE>(a, read_row(a, i), block_nodes);
     if (i == lo) first = w;
     mine += w;
   }
   // exclusive prefix over the threads
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (blockDim.x + 31) / 32;
-  long long inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long n = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += n;
-  }
+  const int inc = warp_inclusive_scan(mine);
   if (lane == 31) tmp[warp] = inc;
   __syncthreads();
-  long long before = inc - mine, total = 0;
+  int before = inc - mine, total = 0;
   for (int w = 0; w < nw; ++w) {
-    if (w < warp) before += tmp[w];
-    total += tmp[w];
+    const int x = tmp[w];
+    before += w < warp ? x : 0;
+    total += x;
   }
   Span s;
-  s.total = total;
-  s.ctas = (int)min((long long)gridDim.x, total);
+  s.ctas = min((int)gridDim.x, total);
+  s.per = s.ctas > 0 ? total / s.ctas : 0;
+  s.extra = total - s.per * s.ctas;
   const int c = blockIdx.x;
-  s.begin = s.end = 0;
-  s.row = 0;
-  s.off = 0;
+  s.begin = s.end = s.row = s.off = 0;
   if (c < s.ctas) {
-    s.begin = total * c / s.ctas;
-    s.end = total * (c + 1) / s.ctas;
+    s.begin = s.per * c + min(c, s.extra);
+    s.end = s.begin + s.per + (c < s.extra ? 1 : 0);
     if (s.begin >= before && s.begin < before + mine) {
-      long long at = s.begin - before;
-      int i = lo;
-      long long w = first;
+      int at = s.begin - before, i = lo, w = first;
       while (at >= w) {
         at -= w;
-        w = weight(++i);
+        w = row_weight<TILE>(a, read_row(a, ++i), block_nodes);
       }
       tmp[32] = i;
       tmp[33] = at;
@@ -117,57 +113,63 @@ __device__ Span my_span(const Rows& a, int block_nodes, long long* tmp) {
   }
   __syncthreads();
   if (c < s.ctas) {
-    s.row = (int)tmp[32];
+    s.row = tmp[32];
     s.off = tmp[33];
   }
-  __syncthreads();
   return s;
 }
 
 // The CTA that has tile x.
-__device__ __forceinline__ int owner(const Span& s, long long x) { return (int)(((x + 1) * s.ctas - 1) / s.total); }
+__device__ __forceinline__ int owner(const Span& s, int x) {
+  const int cut = s.extra * (s.per + 1);
+  return x < cut ? x / (s.per + 1) : s.extra + (x - cut) / s.per;
+}
 
 // One run of tiles of one item, within one CTA.
 struct Segment {
-  int row, hk, block;     // the item
+  int hk, block;          // the item: K/V head and query block
   Row r;
   int t0, t1, tiles;      // key tiles [t0, t1) of the item's `tiles`
-  long long first;        // the item's first tile on the line
+  int first;              // the item's first tile on the line
 };
+
+// Whether the tiles of any call of these sizes can be counted in 31 bits.
+inline bool countable(const Rows& a, int tile, int block_nodes) {
+  const int64_t tiles = (a.max_keys + tile - 1) / tile, blocks = (a.max_nodes + block_nodes - 1) / block_nodes;
+  return (double)tiles * (double)blocks * a.kv_heads * a.rows < 2147483647.0;
+}
 
 // Walks a CTA's segments.
 template <int TILE>
 struct Walk {
   const Rows& a;
-  const Span& s;
-  int block_nodes;
-  long long at;  // next tile on the line
-  int row;
-  long long off;
+  int block_nodes, at, end, row, off, w, nt, nb;  // next tile on the line, ...; the row's weight, tiles, blocks
+  Row r;
   __device__ Walk(const Rows& rows, const Span& span, int bn)
-      : a(rows), s(span), block_nodes(bn), at(span.begin), row(span.row), off(span.off) {}
+      : a(rows), block_nodes(bn), at(span.begin), end(span.end), row(span.row), off(span.off) {
+    if (at < end) load();
+  }
+  __device__ __forceinline__ void load() {
+    r = read_row(a, row);
+    nt = key_tiles<TILE>(r);
+    nb = q_blocks(a, r, block_nodes);
+    w = nt * nb * a.kv_heads;
+  }
   __device__ bool next(Segment& g) {
-    if (at >= s.end) return false;
-    Row r = read_row(a, row);
-    int nt = key_tiles<TILE>(r);
-    long long w = (long long)nt * q_blocks(a, r, block_nodes) * a.kv_heads;
+    if (at >= end) return false;
     while (off >= w) {
       off -= w;
       if (++row >= a.rows) return false;
-      r = read_row(a, row);
-      nt = key_tiles<TILE>(r);
-      w = (long long)nt * q_blocks(a, r, block_nodes) * a.kv_heads;
+      load();
     }
-    const long long item = off / nt;
-    g.row = row;
+    const int item = off / nt;
     g.r = r;
     g.tiles = nt;
-    g.t0 = (int)(off - item * nt);
-    g.t1 = (int)min((long long)nt, g.t0 + (s.end - at));
+    g.t0 = off - item * nt;
+    g.t1 = min(nt, g.t0 + (end - at));
     // the blocks of one K/V head side by side: they read the same keys
-    const int nb = q_blocks(a, r, block_nodes);
-    g.hk = (int)(item / nb);
-    g.block = (int)(item % nb);
+    g.hk = item / nb;
+    g.block = item - g.hk * nb;
     g.first = at - g.t0;
     at += g.t1 - g.t0;
     off += g.t1 - g.t0;
@@ -176,8 +178,10 @@ struct Walk {
 };
 
 // 32 keys' visibility for one query node, bit b for key `key0 + b`: every key
-// below the context, then the nodes its mask names.
-__device__ __forceinline__ uint32_t visible32(const int64_t* mask, int words, const Row& r, int key0) {
+// below the context, then the nodes its mask names; word(i): the mask's i-th 32
+// bits (i < 2 words).
+template <typename F>
+__device__ __forceinline__ uint32_t visible32(F word, int words, const Row& r, int key0) {
   if (r.slot < 0) return 0u;
   const int d = key0 - r.ctx;
   if (d <= -32) return 0xffffffffu;
@@ -185,9 +189,8 @@ __device__ __forceinline__ uint32_t visible32(const int64_t* mask, int words, co
   // node bits [max(d, 0), d + 32) of the mask, nodes past the tree never
   const int n0 = max(d, 0), sh = n0 - d;
   if (n0 < r.nodes) {
-    const uint32_t* m = reinterpret_cast<const uint32_t*>(mask);
     const int w = n0 >> 5, b = n0 & 31, nw = 2 * words;
-    const uint32_t lo = w < nw ? __ldg(m + w) : 0u, up = w + 1 < nw ? __ldg(m + w + 1) : 0u;
+    const uint32_t lo = w < nw ? word(w) : 0u, up = w + 1 < nw ? word(w + 1) : 0u;
     uint32_t x = __funnelshift_r(lo, up, b);
     const int left = r.nodes - n0;
     if (left < 32) x &= (1u << left) - 1u;
