@@ -107,6 +107,93 @@ __device__ __forceinline__ void softmax_tile(uint32_t lane_base, uint32_t s_col,
   row.l += (a + b) + (c + d);
 }
 
+// The same in rolled loops of 32 columns, the scores read twice: a quarter of the
+// code and of the registers.  For kernels whose warps come back to a tile after
+// much other code: there the instructions' own way through the caches counts
+// (the token tree kernel lost a third of its time to it).
+template <int HD>
+__device__ __forceinline__ void softmax_tile_small(uint32_t lane_base, uint32_t s_col, uint32_t o_col, float sl2,
+                                                   bool first, bool masked, uint32_t vis0, uint32_t vis1, uint32_t vis2,
+                                                   uint32_t vis3, RowState& row, uint32_t half0) {
+  const uint32_t sa = lane_base + s_col;
+  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int c = 0; c < kKeys; c += 32) {
+    uint32_t u[32];
+    float* f = reinterpret_cast<float*>(u);
+    tmem_ld32(sa + c, u);
+    tmem_wait_ld();
+    if (masked) {
+      // hidden scores become -inf where they stand, for the second pass
+#pragma unroll
+      for (int i = 0; i < 32; ++i) f[i] = vis0 >> i & 1u ? f[i] : -INFINITY;
+      tmem_st32(sa + c, u);
+      vis0 = vis1;
+      vis1 = vis2;
+      vis2 = vis3;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) m4[y] = fmax3_nan(m4[y], f[i + y], f[i + 4 + y]);
+    }
+  }
+  if (masked) tmem_wait_st();
+  const float mx = fmax3_nan(fmax3_nan(m4[0], m4[1], m4[2]), m4[3], m4[3]) * sl2;
+  // a NaN or +inf among the scores: the row's result is NaN
+  if (!(mx < INFINITY)) row.l = __int_as_float(0x7fffffff);
+  float corr = 1.f;
+  if (mx > row.m + 8.f) {
+    corr = ex2(row.m - mx);  // 0 from -inf
+    row.m = mx;
+  }
+  row.l *= corr;
+  if (!first && __any_sync(0xffffffffu, corr != 1.f)) {
+    // every product issued before these scores has retired (their commit
+    // covers it), so the output can be rescaled in place
+#pragma unroll 1
+    for (int c = 0; c < HD; c += 16) {
+      uint32_t o[16];
+      tmem_ld16(lane_base + o_col + c, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+      tmem_st16(lane_base + o_col + c, o);
+    }
+  }
+  const float neg = row.m == -INFINITY ? 0.f : -row.m;
+  const uint64_t sc2 = pack2(sl2, sl2), neg2 = pack2(neg, neg);
+  uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll 1
+  for (int c = 0; c < kKeys; c += 32) {
+    uint32_t u[32], p[16];
+    const float* f = reinterpret_cast<const float*>(u);
+    tmem_ld32(sa + c, u);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float lo, hi;
+      unpack2(fma2(pack2(f[2 * i], f[2 * i + 1]), sc2, neg2), lo, hi);
+      lo = ex2(lo);
+      hi = ex2(hi);
+      sum[i & 1] = add2(sum[i & 1], pack2(lo, hi));
+      p[i] = pack_bf16(lo, hi);
+    }
+    // over columns that have been read: chunk c's weights lie under chunk c / 2
+    tmem_st16(sa + c / 2, p);
+    if (c & 32) {
+      tmem_wait_st();
+      fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(half0 + (c >> 6) * 8);
+    }
+  }
+  float a, b, c, d;
+  unpack2(sum[0], a, b);
+  unpack2(sum[1], c, d);
+  row.l += (a + b) + (c + d);
+}
+
 // 32 columns of an output row, scaled and rounded; vec: the row is 16-byte aligned.
 __device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const float* o, float inv, bool vec) {
 #pragma unroll
@@ -137,6 +224,7 @@ __device__ __forceinline__ bool clear_nonfinite(uint4* v, int n) {
   const int lane = threadIdx.x & 31;
   const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
   bool bad = false;
+#pragma unroll 1
   for (int i = lane; i < n; i += 256) {
     // 0 x value, summed: NaN if any value is not finite, else a zero
     __nv_bfloat162 z = zero;
@@ -154,6 +242,7 @@ __device__ __forceinline__ bool clear_nonfinite(uint4* v, int n) {
   bad = __any_sync(0xffffffffu, bad);
   if (bad) {
     uint32_t* w = reinterpret_cast<uint32_t*>(v);
+#pragma unroll 1
     for (int i = lane; i < 4 * n; i += 32) {
       uint32_t x = w[i];
       if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;

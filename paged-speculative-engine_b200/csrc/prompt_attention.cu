@@ -262,9 +262,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (guarded) ++g;
           return true;
         };
-        for (int e = e0; run && e < e1; ++e) {
+#pragma unroll 1
+#pragma unroll 1
+    for (int e = e0; run && e < e1; ++e) {
           const TcItem it = decode(a, e, tpt);
           if (it.n_max == 0) continue;
+#pragma unroll 1
           for (int j = 0; run && j < it.n_max; ++j)
             run = load(&tmk, it.hk, it.tok0 + j * 128, false) && load(&tmv, it.hk, it.tok0 + j * 128, j >= it.guard0);
         }
@@ -273,6 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // -------------------------------------------------------------- queries
       if (lane == 0) {
         int nq = 0;
+#pragma unroll 1
         for (int e = e0; e < e1; ++e) {
           const TcItem it = decode(a, e, tpt);
           if (it.n_max == 0) continue;
@@ -280,8 +284,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int streams = it.n[1] > 0 ? 2 : 1;
           last_bar[NS] = nq & 1;
           mbar_expect_tx(q_full, streams * kHalves * tpt * a.group * 128);
+#pragma unroll 1
           for (int s = 0; s < streams; ++s)
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < kHalves; ++h)
               tma_load_3d(q_s + s * kTileBytes + h * kHalfBytes, &tmq, h * 64, it.hk * a.group,
                           it.tok0 + it.w0 + s * tpt, q_full);
@@ -306,7 +311,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           fill ^= 1;
         }
       };
-      for (int e = e0; run && e < e1; ++e) {
+#pragma unroll 1
+    for (int e = e0; run && e < e1; ++e) {
         const TcItem it = decode(a, e, tpt);
         if (it.n_max == 0) continue;
         const int n0 = it.n[0], n1 = it.n[1], n = it.n_max;
@@ -369,10 +375,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // -------------------------------------------------------------- guard
       int c = 0, g = 0, items = 0;
       bool run = true;
-      for (int e = e0; run && e < e1; ++e) {
+#pragma unroll 1
+    for (int e = e0; run && e < e1; ++e) {
         const TcItem it = decode(a, e, tpt);
         if (it.n_max == 0) continue;
         int marks = 0;
+#pragma unroll 1
         for (int j = it.guard0; j < it.n_max; ++j, ++g) {
           if (!mbar_wait_warp(&guard_full[g % kGuards], (g / kGuards) & 1, vabort)) {
             run = false;
@@ -398,6 +406,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int rt = r / a.group, rg = r - rt * a.group;
     int nt = 0, items = 0, no = 0;  // tiles, items and outputs of this stream
     bool run = true;
+#pragma unroll 1
     for (int e = e0; run && e < e1; ++e) {
       const TcItem it = decode(a, e, tpt);
       if (it.n_max == 0) continue;
@@ -409,6 +418,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool any_valid = __any_sync(0xffffffffu, valid);
       tile::RowState row;
       row.reset();
+#pragma unroll 1
       for (int j = 0; j < it.n[s]; ++j, ++nt) {
         if (!mbar_wait_warp(&s_full[s], nt & 1, vabort)) {
           run = false;

@@ -43,6 +43,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait that also gives up once another role of the CTA has.  (Each try
 // suspends the thread in hardware for a while.  The loop is this short because
 // it stands in some thirty places: kernels whose warps walk different code
@@ -169,13 +179,14 @@ __device__ __forceinline__ void mma_ts(uint32_t elected, uint32_t d, uint32_t a,
       : "memory");
 }
 // The barrier's arrival waits for every tcgen05 operation the elected thread issued before.
-__device__ __forceinline__ void mma_commit(uint32_t elected, uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t elected, uint32_t bar) {
   asm volatile(
       "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
-      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(su32(bar)),
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
       "r"(elected)
       : "memory");
 }
+__device__ __forceinline__ void mma_commit(uint32_t elected, uint64_t* bar) { mma_commit(elected, su32(bar)); }
 
 // S = Q K^T (M = N = 128) over head_dim HD: both operands as HD / 64 column
 // halves of 16 KB.

@@ -15,8 +15,8 @@ namespace pse {
 namespace tree {
 
 struct Cut;
-constexpr int kMaxCtas = 2 * kNumSMs;
-constexpr size_t kCutBytes = 8192;  // a Cut per CTA
+constexpr int kMaxWorkers = 2 * kNumSMs;
+constexpr size_t kCutBytes = 8192;  // a Cut per worker
 
 struct Args {
   Rows rows;
@@ -33,17 +33,17 @@ struct Args {
   int words;
   int block_nodes;
   float scale_log2;
-  Cut* cuts;  // [ctas]
-  float* parts;      // [ctas][2][part_rows][hd + 2]
+  Cut* cuts;     // [workers]
+  float* parts;  // [workers][2][part_rows][hd + 2]
   int part_rows;
   int32_t* status;
   bool out_vec;  // output rows are 16-byte aligned
 };
 
-// Partial results of cut items: per CTA two blocks of `part_rows` rows of hd
-// columns, then a (maximum, sum) per row.  A CTA's first segment, if it begins
+// Partial results of cut items: per worker two blocks of `part_rows` rows of hd
+// columns, then a (maximum, sum) per row.  A worker's first segment, if it begins
 // inside an item, uses the first block; a segment that begins an item and does
-// not end it, necessarily the CTA's last, uses the second.
+// not end it, necessarily the worker's last, uses the second.
 __device__ __forceinline__ float* part(const Args& a, int cta, bool starts_item) {
   return a.parts + ((int64_t)cta * 2 + (starts_item ? 1 : 0)) * a.part_rows * (a.hd + 2);
 }
@@ -52,16 +52,16 @@ __device__ __forceinline__ float* part_stats(const Args& a, float* block, int r)
   return block + (int64_t)a.part_rows * a.hd + 2 * r;
 }
 
-// What the join needs of the item that CTA c begins and does not end.
+// What the join needs of the item that worker c begins and does not end.
 struct Cut {
-  int last;    // the item's last CTA (-1: CTA c cuts nothing)
+  int last;    // the item's last worker (-1: worker c cuts nothing)
   int node0;   // its first query node
   int nodes;   // and their number
   int hk;
 };
 
 // A warp per row of a cut item, lanes over the columns: the parts are summed in
-// the order of their CTAs.
+// the order of their workers.
 template <typename T, int PER>
 __global__ void join_kernel(const Args a, int tile_rows, int tile_pitch) {
   pdl_wait();
@@ -108,10 +108,10 @@ __global__ void join_kernel(const Args a, int tile_rows, int tile_pitch) {
 }
 
 template <typename T>
-int launch_join(const Args& a, int ctas, int max_nodes, int tile_rows, int tile_pitch, cudaStream_t s) {
+int launch_join(const Args& a, int workers, int max_nodes, int tile_rows, int tile_pitch, cudaStream_t s) {
   const int rows = (max_nodes < a.block_nodes ? max_nodes : a.block_nodes) * a.rows.group;
   const int warps = rows < 16 ? rows : 16;
-  const dim3 grid(ctas, ceil_div(rows, warps)), block(32 * warps);
+  const dim3 grid(workers, ceil_div(rows, warps)), block(32 * warps);
   const cudaError_t e = a.hd <= 64    ? launch_pdl(join_kernel<T, 2>, grid, block, 0, s, a, tile_rows, tile_pitch)
                         : a.hd <= 128 ? launch_pdl(join_kernel<T, 4>, grid, block, 0, s, a, tile_rows, tile_pitch)
                                       : launch_pdl(join_kernel<T, 8>, grid, block, 0, s, a, tile_rows, tile_pitch);
@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
   extern __shared__ float smem[];
   __shared__ int tmp[36];
   constexpr int BQ = 16 * RPT, TILE = simt::BK;
-  const Span span = my_span<TILE>(a.rows, a.block_nodes, tmp);
+  Span span;
+  const Split split = my_span<TILE>(a.rows, a.block_nodes, tmp, span);
   Cut cut{-1, 0, 0, 0};
   simt::Tile<RPT, NC> t;
   t.init(smem, a.hd);
@@ -134,7 +135,8 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
   };
   const bool qvec = aligned(a.q, a.q_tok, a.q_head);
   const bool kvec = aligned(a.k_pool, hd, hd), vvec = aligned(a.v_pool, hd, hd);
-  Walk<TILE> walk(a.rows, span, a.block_nodes);
+  Walk<TILE> walk;
+  walk.start(a.rows, span, a.block_nodes);
   Segment g;
   while (walk.next(g)) {
     // rows of the block: (node, group head), node-major; a group above BQ heads
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
         if (r >= nr || k0 + key >= keys) return false;
         const uint32_t* m = reinterpret_cast<const uint32_t*>(a.masks + (int64_t)(g.r.n0 + node0 + r / group) * a.words);
         const auto word = [&](int i) { return __ldg(m + i); };
-        return (visible32(word, a.words, g.r, k0 + (key & ~31)) >> (key & 31) & 1u) != 0u;
+        return (visible32(word, a.words, g.r.slot, g.r.ctx, g.r.nodes, k0 + (key & ~31)) >> (key & 31) & 1u) != 0u;
       });
     }
     T* out = reinterpret_cast<T*>(a.out);
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
     const bool whole = g.t0 == 0 && g.t1 == g.tiles;
     float* mine = part(a, blockIdx.x, g.t0 == 0);
     if (g.t0 == 0 && !whole)
-      cut = Cut{owner(span, g.first + g.tiles - 1), g.r.n0 + node0, min(a.block_nodes, g.r.nodes - node0), g.hk};
+      cut = Cut{owner(split, g.first + g.tiles - 1), g.r.n0 + node0, min(a.block_nodes, g.r.nodes - node0), g.hk};
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       const float L = t.row_sum(i);
@@ -242,70 +244,84 @@ int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
   a.block_nodes = 16 * rpt / a.rows.group;
   a.part_rows = 16 * rpt;
   if (!countable(a.rows, simt::BK, a.block_nodes)) return PSE_EINVAL;
-  const int rc = rpt == 1 ? simt_nc<T, 1>(a, kMaxCtas, s) : simt_nc<T, 4>(a, kMaxCtas, s);
-  return rc == PSE_OK ? launch_join<T>(a, kMaxCtas, max_nodes, a.part_rows, a.part_rows, s) : rc;
+  const int rc = rpt == 1 ? simt_nc<T, 1>(a, kMaxWorkers, s) : simt_nc<T, 4>(a, kMaxWorkers, s);
+  return rc == PSE_OK ? launch_join<T>(a, kMaxWorkers, max_nodes, a.part_rows, a.part_rows, s) : rc;
 }
 
 // ---------------------------------------------------------------- tensor cores
-// bf16 pools, head_dim 64 or 128, pages of 16, 32, 64 or 128 tokens.  One CTA
-// per multiprocessor walks its tiles of the line (tree_partition.cuh).  A query
-// tile is 128 rows, (node, group head) node-major.  Two softmax streams:
-//   NQ = 2 (more than 128 rows per K/V head): two query tiles share every K/V
-//          tile, one per stream;
-//   NQ = 1: both streams hold the same query tile and take the key tiles in
-//          turn, each with an output of its own; at a segment's end the two are
-//          joined, each stream's warps writing half of the columns (warps w and
-//          w + 4 reach the same TMEM lanes, so no output crosses shared memory).
-// Either way one stream's softmax runs beside the other's products.  Warps:
-//   0-3, 4-7  the streams' softmax (attention_tile.cuh), a thread per row
-//   8         K and V pages by TMA into a ring of 128-key slots
-//   9         the products
-//   10        clears V tiles that hold nodes (or what stands after them) of
-//             infinities and NaN before the product, as in prompt_attention.cu
-//   11        Q tiles, so that the ring runs on into the next segment
+// bf16 pools, head_dim 64 or 128, pages of 16, 32, 64 or 128 tokens.  A query
+// tile is 128 rows, (node, group head) node-major, and has a stream: four softmax
+// warps with 256 columns of tensor memory.
+//   NQ = 1 (at most 128 rows per K/V head): a CTA has one stream, and a
+//          multiprocessor two CTAs, each a worker of its own: while one's softmax
+//          runs or its output is written, the other loads and multiplies;
+//   NQ = 2: one CTA with two streams, the two query tiles of an item, which share
+//          every K/V tile (the second one idles through a block whose last nodes
+//          fill one tile).
+// Warps (h = 4 NQ):
+//   0 .. h - 1  the softmax (attention_tile.cuh), a thread per row, and the output
+//   h, h + 4    K, and V pages by TMA into a ring of 128-key slots (a copy takes
+//               its warp some 50 clocks to issue, and a tile of 16-token pages is
+//               16 copies)
+//   h + 1       the products
+//   h + 2       clears V tiles that hold nodes (or what stands after them) of
+//               infinities and NaN before the product, as in prompt_attention.cu
+//   h + 3       Q tiles, so that the ring runs on into the next segment, and what
+//               the softmax and product warps have to know of it (Seg)
 using namespace t5;
 
-constexpr int kTcThreads = 384;
 constexpr int kHalfBytes = 128 * 128;
 constexpr int kGuards = 8;
-constexpr uint32_t kColS = 0, kColO = 256;
 
+template <int NQ>
+__host__ __device__ constexpr int n_threads() { return 32 * (4 * NQ + 5); }
+// two CTAs share a multiprocessor's 227 KB when NQ = 1: at head_dim 128 a K and a
+// V tile each, whose loads still pass behind the other tile's softmax
 template <int HD, int NQ>
-__host__ __device__ constexpr int n_slots() { return HD == 128 ? 5 : 10; }
+__host__ __device__ constexpr int n_slots() { return HD == 128 ? (NQ == 1 ? 2 : 5) : (NQ == 1 ? 5 : 10); }
 
 template <int HD, int NQ>
 constexpr size_t tc_smem_bytes() {
-  return 1024 + (size_t)(NQ + n_slots<HD, NQ>()) * 128 * HD * 2 + 640 + (NQ == 1 ? 4096 : 0);
+  return 1024 + (size_t)(NQ + n_slots<HD, NQ>()) * 128 * HD * 2 + 512;
 }
 
+// A segment as the softmax and product warps read it from shared memory when
+// they need it: held in registers it would not fit beside a row of scores.
+struct Seg {
+  int q0, nodes;           // the block's first query, and its nodes
+  int hk, slot, ctx, row_nodes;
+  int t0, t1, tiles, first;
+  int g0;                  // tiles from here on hold keys that some node may not see
+};
+constexpr int kSegs = 4;
+
 template <int HD, int NQ>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                    const __grid_constant__ CUtensorMap tmv, const Args a) {
-  constexpr int NS = n_slots<HD, NQ>();
+  constexpr int NS = n_slots<HD, NQ>(), kHelp = 4 * NQ;
   constexpr int kTileBytes = 128 * HD * 2, kHalves = HD / 64;
-  constexpr int HDS = NQ == 1 ? HD / 2 : HD;  // output columns of a softmax thread
+  constexpr uint32_t kColO = 128 * NQ, kTmem = 256 * NQ;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int span_tmp[36];
+  __shared__ Seg segs[kSegs];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_s = smem;                     // [NQ][128 x HD]
-  uint8_t* ring = q_s + NQ * kTileBytes;   // [NS][128 x HD]
+  uint8_t* q_s = smem;                      // [NQ][128 x HD]
+  uint8_t* ring = q_s + NQ * kTileBytes;    // [NS][128 x HD]: K and V tiles in turn
   uint64_t* slot_full = reinterpret_cast<uint64_t*>(ring + NS * kTileBytes);
   uint64_t* slot_empty = slot_full + NS;
-  uint64_t* guard_full = slot_empty + NS;  // [kGuards] a guarded V tile landed
+  uint64_t* guard_full = slot_empty + NS;   // [kGuards] a guarded V tile landed
   uint64_t* q_full = guard_full + kGuards;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;          // [2]
-  uint64_t* p_half = s_full + 2;           // [2][2]
-  uint64_t* o_full = p_half + 4;           // [2]
-  uint64_t* o_empty = o_full + 2;          // [2] (NQ = 1: one for both outputs)
-  uint64_t* x_bar = o_empty + 2;           // [4] the streams' warps of one lane quarter (NQ = 1)
-  uint64_t* final_bar = x_bar + 4;
+  uint64_t* s_full = q_empty + 1;           // [NQ] a stream's scores stand
+  uint64_t* p_half = s_full + 2;            // [NQ][2] half of its weights stand
+  uint64_t* o_full = p_half + 4;            // [NQ] its last product of the segment retired
+  uint64_t* o_empty = o_full + 2;           // [NQ] its output has been read
+  uint64_t* final_bar = o_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  int* poison = abort_flag + 1;            // [kGuards]
-  int* last_bar = poison + kGuards;        // [NS + 1]
-  float* ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(slot_full) + 640);  // [2 segments][2 streams][128][2]
+  int* poison = abort_flag + 1;             // [kGuards] segments' marked tiles, bit j: tile g0 + j
+  int* last_bar = poison + kGuards;         // [NS + 1] per slot (and Q): barrier and parity of its last copy
   volatile int* vabort = abort_flag;
 
   const int tid = threadIdx.x, lane = tid & 31;
@@ -318,21 +334,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int i = 0; i < kGuards; ++i) mbar_init(&guard_full[i], 1);
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NQ; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&p_half[2 * s], 4);
       mbar_init(&p_half[2 * s + 1], 4);
       mbar_init(&o_full[s], 1);
-      mbar_init(&o_empty[s], NQ == 1 ? 8 : 4);
+      mbar_init(&o_empty[s], 4);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&x_bar[i], 2);
     mbar_init(final_bar, 1);
     *abort_flag = 0;
     for (int i = 0; i <= NS; ++i) last_bar[i] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(512));
+  if (warp == kHelp + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmem));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   fence_before();
@@ -340,233 +355,300 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
-  const Span span = my_span<128>(a.rows, a.block_nodes, span_tmp);
+  Span span;
+  const Split split = my_span<128>(a.rows, a.block_nodes, span_tmp, span);
   const int group = a.rows.group, tpt = 128 / group;
-  Walk<128> walk(a.rows, span, a.block_nodes);
-  Segment g;
-  // tiles of a segment that each stream takes
-  auto counts = [&](const Segment& x, int* n) {
-    const int nt = x.t1 - x.t0;
-    if (NQ == 1) {
-      n[0] = (nt + 1) >> 1;
-      n[1] = nt >> 1;
-    } else {
-      n[0] = nt;
-      n[1] = x.block * a.block_nodes + tpt < x.r.nodes ? nt : 0;
-    }
-  };
-  // tiles from here on hold keys that some node may not see
   auto guard_from = [&](const Segment& x) { return max(x.t0, x.r.slot < 0 ? 0 : x.r.ctx >> 7); };
-  // ring positions of a segment's K and V tiles i
-  auto k_at = [](int i) { return 2 * i; };
-  auto v_at = [](int i) { return 2 * i + 1; };
+  bool run = true;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8) {
+  if (warp < kHelp) {
+    // ---------------------------------------------------------------- softmax
+    const int s = NQ == 1 ? 0 : warp >> 2, r = tid & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const int rt = r / group, rg = r - rt * group;
+    const int total = span.end - span.begin;
+    int done = 0, items = 0;  // tiles and segments of this stream
+    int cut = -1;             // Cut::last of the item that the worker's last segment begins
+#pragma unroll 1
+    while (run && done < total) {
+      // a segment is known here once its first scores stand
+      run = mbar_wait_warp(&s_full[s], done & 1, vabort);
+      if (!run) break;
+      const Seg& x = segs[items % kSegs];
+      const int node = s * tpt + rt;  // within the block
+      const bool valid = rt < tpt && node < x.nodes;
+      const bool any_valid = __any_sync(0xffffffffu, valid);
+      const uint32_t* mask =
+          reinterpret_cast<const uint32_t*>(a.masks) + (int64_t)(x.q0 + (valid ? node : 0)) * (2 * a.words);
+      // the first word of the mask (all of it, up to 64 nodes)
+      const uint2 head = __ldg(reinterpret_cast<const uint2*>(mask));
+      auto bits = [&](int key0) {
+        return visible32([&](int i) { return i == 0 ? head.x : i == 1 ? head.y : __ldg(mask + i); }, a.words, x.slot,
+                         x.ctx, x.row_nodes, key0);
+      };
+      tile::RowState row;
+      row.reset();
+      const int t0 = x.t0, t1 = x.t1;
+#pragma unroll 1
+      for (int t = t0; t < t1; ++t, ++done) {
+        const bool masked = t >= x.g0;
+        uint32_t vis[4] = {0u, 0u, 0u, 0u};
+        if (masked && valid) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) vis[y] = bits(t * 128 + 32 * y);
+        }
+        if (t > t0) run = mbar_wait_warp(&s_full[s], done & 1, vabort);
+        if (!run) break;
+        fence_after();
+        if (!any_valid) {
+          // no row of this warp is anyone's: its weights may be anything
+          if (lane == 0) {
+            mbar_arrive(&p_half[2 * s]);
+            mbar_arrive(&p_half[2 * s + 1]);
+          }
+          continue;
+        }
+        tile::softmax_tile_small<HD>(lane_base, s * 128, kColO + s * 128, a.scale_log2, t == t0, masked, vis[0], vis[1],
+                                     vis[2], vis[3], row, su32(&p_half[2 * s]));
+      }
+      if (!run || !mbar_wait_warp(&o_full[s], items & 1, vabort)) break;
+      fence_after();
+      const int marks = x.g0 < t1 ? poison[items % kGuards] : 0;
+      const bool whole = t0 == 0 && t1 == x.tiles;
+      // a row whose weights are all zero (nothing visible, or every score -inf) gives zero
+      const float inv = whole ? (row.l == 0.f ? 0.f : 1.f / row.l) : 1.f;
+      float* mine = part(a, blockIdx.x, t0 == 0);
+      const int prow = s * 128 + r;
+      if (t0 == 0 && !whole) {
+        cut = owner(split, x.first + x.tiles - 1);
+        if (tid == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(cut, x.q0, x.nodes, x.hk);
+      }
+      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + (int64_t)(x.q0 + node) * a.o_tok +
+                           (int64_t)(x.hk * group + rg) * a.o_head;
+#pragma unroll 1
+      for (int col = 0; col < HD; col += 32) {
+        uint32_t u[32];
+        float* o = reinterpret_cast<float*>(u);
+        if (any_valid) {
+          tmem_ld32(lane_base + kColO + s * 128 + col, u);
+          tmem_wait_ld();
+        }
+        if (marks && valid) {
+          const int keys = min(x.ctx + x.row_nodes, t1 * 128);
+#pragma unroll 1
+          for (int key = x.g0 * 128; key < keys; ++key) {
+            if (!(marks >> min((key >> 7) - x.g0, 31) & 1) || !(bits(key & ~31) >> (key & 31) & 1u)) continue;
+            const int bi = key / a.block_size;
+            if (x.slot < 0 || bi >= min(a.nblocks[x.slot], a.max_blocks)) continue;
+            const int blk = a.block_table[(int64_t)x.slot * a.max_blocks + bi];
+            if (blk < 0 || blk >= a.num_blocks) continue;
+            const __nv_bfloat16* v =
+                reinterpret_cast<const __nv_bfloat16*>(a.v_pool) +
+                (((int64_t)blk * a.rows.kv_heads + x.hk) * a.block_size + key % a.block_size) * HD + col;
+#pragma unroll
+            for (int y = 0; y < 32; ++y) {
+              const float f = __bfloat162float(v[y]);
+              if (!isfinite(f)) o[y] += f;
+            }
+          }
+        }
+        if (valid && whole) {
+          tile::store_row32(dst + col, o, inv, a.out_vec);
+        } else if (valid) {
+          float4* p = reinterpret_cast<float4*>(part_row(a, mine, prow) + col);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) __stcg(p + y, make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]));
+        }
+      }
+      if (!whole && valid) __stcg(reinterpret_cast<float2*>(part_stats(a, mine, prow)), make_float2(row.m, row.l));
+      // the output and the segment's description have been read
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[s]);
+      ++items;
+    }
+    if (cut < 0 && tid == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(-1, 0, 0, 0);
+  } else if (warp == kHelp + 1) {
+    // ---------------------------------------------------------------- products
+    const uint32_t el = elect_one();
+    const uint32_t full0 = su32(slot_full), empty0 = su32(slot_empty), ring0 = su32(ring), q0 = su32(q_s);
+    const uint32_t part0 = su32(p_half);
+    int slot = 0;                  // next slot of the ring, and the parity of its fill
+    uint32_t fill = 0;
+    uint32_t parts = 0, outs = 3;  // per stream (bit): parity of its next weights, of its last output's reading
+    int segment = 0;
+    auto next_slot = [&](int& i, uint32_t& par) {
+      i = slot;
+      par = fill;
+      if (++slot == NS) {
+        slot = 0;
+        fill ^= 1;
+      }
+    };
+#pragma unroll 1
+    for (int left = span.end - span.begin; run && left > 0;) {
+      int k, v = 0, nt = 0;
+      uint32_t kp, vp = 0;
+      // step i: the values of tile i, then the scores of tile i + 1, stream by stream
+#pragma unroll 1
+      for (int i = -1; run && i < nt; ++i) {
+        if (i >= 0) next_slot(v, vp);
+        const bool more = i + 1 < nt || i < 0;
+        const uint32_t vbar = full0 + 8 * v;
+        if (more) {
+          next_slot(k, kp);
+        } else {
+          k = v;
+          kp = vp;
+        }
+        const uint32_t kbar = full0 + 8 * k;
+        if (i < 0) {
+          run = mbar_wait3_warp(su32(q_full), segment & 1, kbar, kp, kbar, kp, vabort);
+          if (!run) break;
+          const Seg& x = segs[segment++ % kSegs];
+          nt = x.t1 - x.t0;
+          left -= nt;
+        }
+#pragma unroll 1
+        for (int s = 0; run && s < NQ; ++s) {
+          const uint32_t s_col = tmem + s * 128, o_col = tmem + kColO + s * 128;
+          if (i >= 0) {
+            const uint32_t part = part0 + 16 * s, par = parts >> s & 1u;
+            // the output of the segment before has been read
+            if (i == 0) run = mbar_wait_warp(&o_empty[s], outs >> s & 1u, vabort);
+            // (at two slots the next K waits for this tile's V to leave its own)
+            run = run && mbar_wait3_warp(part, par, vbar, vp, vbar, vp, vabort);
+            if (!run) break;
+            fence_after();
+            issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 0, i == 0);
+            run = mbar_wait3_warp(part + 8, par, kbar, kp, kbar, kp, vabort);
+            if (!run) break;
+            fence_after();
+            issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 1, false);
+            parts ^= 1u << s;
+            if (!more) {
+              mma_commit(el, &o_full[s]);
+              outs ^= 1u << s;
+            }
+          }
+          if (more) {
+            fence_after();
+            issue_scores<HD>(el, s_col, q0 + s * kTileBytes, ring0 + k * kTileBytes);
+            mma_commit(el, &s_full[s]);
+          }
+        }
+        if (!run) break;
+        if (i >= 0) mma_commit(el, empty0 + 8 * v);
+        if (more) mma_commit(el, empty0 + 8 * k);
+        if (i + 2 == nt) mma_commit(el, q_empty);
+      }
+    }
+    mma_commit(el, final_bar);
+  } else {
+    Walk<128> walk;
+    walk.start(a.rows, span, a.block_nodes);
+    Segment g;
+    if (warp == kHelp || warp == kHelp + 4) {
       // -------------------------------------------------------------- pages
-      const int bs = a.block_size, ppt = 128 / bs, oob = a.num_blocks * a.rows.kv_heads * bs;
+      const bool is_v = warp != kHelp;
+      const int bs = a.block_size, ppt = 128 / bs, tpc = 32 / ppt, oob = a.num_blocks * a.rows.kv_heads * bs;
       const uint32_t el = elect_one();
       const uint32_t empty0 = su32(slot_empty), full0 = su32(slot_full), guard0 = su32(guard_full), ring0 = su32(ring);
-      int gd = 0, slot = 0;
+      const CUtensorMap* map = is_v ? &tmv : &tmk;
+      int gd = 0, slot = is_v ? 1 : 0;
       uint32_t fill = 0;
-      bool run = true;
+#pragma unroll 1
       while (run && walk.next(g)) {
-        const int nt = g.t1 - g.t0, g0 = guard_from(g);
-        const int keys = g.r.ctx + g.r.nodes;
+        const int g0 = guard_from(g), keys = g.r.ctx + g.r.nodes;
         const int32_t* table = a.block_table + (int64_t)max(g.r.slot, 0) * a.max_blocks;
         const int held = g.r.slot >= 0 ? min(a.nblocks[g.r.slot], a.max_blocks) : 0;
-        // lanes hold the pool rows of 32 pages (32 / ppt tiles), the next 32 on their way
+        // the pool rows of 32 pages (32 / ppt tiles), a page per lane, and of the next 32
         auto page = [&](int j) -> int {
           const int pi = g.t0 * ppt + j;
-          if (j >= nt * ppt || pi >= held || pi * bs >= keys) return oob;
+          if (pi >= g.t1 * ppt || pi >= held || pi * bs >= keys) return oob;
           const int b = __ldg(table + pi);
           return b >= 0 && b < a.num_blocks ? (b * a.rows.kv_heads + g.hk) * bs : oob;
         };
         int cur = page(lane), nxt = page(32 + lane);
-        const int tpc = 32 / ppt;  // tiles per chunk
-        for (int i = 0; run && i < nt; ++i) {
-          const int src = (i % tpc) * ppt;
+#pragma unroll 1
+        for (int t = g.t0; t < g.t1; ++t) {
+          const int i = t - g.t0, src = (i & (tpc - 1)) * ppt;
           if (i > 0 && src == 0) {
             cur = nxt;
             nxt = page(32 * (i / tpc + 1) + lane);
           }
-          // the tile's K, then its V, page by page with operands uniform over the warp
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            run = run && mbar_wait_warp(empty0 + 8 * slot, fill ^ 1, vabort);
-            if (!run) break;
-            const bool guarded = kv == 1 && g.t0 + i >= g0;
-            const uint32_t bar = guarded ? guard0 + 8 * (gd % kGuards) : full0 + 8 * slot;
-            if (el) {
-              last_bar[slot] = guarded ? (NS + gd % kGuards) * 2 + ((gd / kGuards) & 1) : slot * 2 + (int)fill;
-              mbar_expect_tx(bar, kTileBytes);
-            }
-            uint32_t dst = ring0 + slot * kTileBytes;
-            for (int p = 0; p < ppt; ++p, dst += bs * 128) {
-              const int y = __shfl_sync(0xffffffffu, cur, src + p);
-#pragma unroll
-              for (int h = 0; h < kHalves; ++h) tma_load_2d(el, dst + h * kHalfBytes, kv ? &tmv : &tmk, h * 64, y, bar);
-            }
-            if (guarded) ++gd;
-            if (++slot == NS) {
-              slot = 0;
-              fill ^= 1;
-            }
+          run = mbar_wait_warp(empty0 + 8 * slot, fill ^ 1, vabort);
+          if (!run) break;
+          const bool guarded = is_v && t >= g0;
+          const uint32_t bar = guarded ? guard0 + 8 * (gd % kGuards) : full0 + 8 * slot;
+          if (el) {
+            last_bar[slot] = guarded ? (NS + gd % kGuards) * 2 + ((gd / kGuards) & 1) : slot * 2 + (int)fill;
+            mbar_expect_tx(bar, kTileBytes);
           }
-        }
-      }
-    } else if (warp == 11) {
-      // -------------------------------------------------------------- queries
-      if (lane == 0) {
-        int nq = 0;
-        while (walk.next(g)) {
-          if (!mbar_wait(q_empty, (nq & 1) ^ 1, vabort)) break;
-          int n[2];
-          counts(g, n);
-          const int tiles = NQ == 2 && n[1] > 0 ? 2 : 1;
-          last_bar[NS] = nq & 1;
-          mbar_expect_tx(q_full, tiles * kHalves * tpt * group * 128);
-          for (int s = 0; s < tiles; ++s)
+          int y[8];
+#pragma unroll
+          for (int p = 0; p < 8; ++p) y[p] = __shfl_sync(0xffffffffu, cur, (src + p) & 31);
+          const uint32_t dst = ring0 + slot * kTileBytes;
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            if (p >= ppt) break;
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
-              tma_load_3d(q_s + s * kTileBytes + h * kHalfBytes, &tmq, h * 64, g.hk * group,
-                          g.r.n0 + g.block * a.block_nodes + s * tpt, q_full);
-          ++nq;
-        }
-      }
-    } else if (warp == 9) {
-      // -------------------------------------------------------------- products
-      const uint32_t el = elect_one();
-      const uint32_t full0 = su32(slot_full), ring0 = su32(ring), q0 = su32(q_s), part0 = su32(p_half);
-      int slot = 0;                  // next slot of the ring, and the parity of its fill
-      uint32_t fill = 0;
-      uint32_t parts = 0, outs = 3;  // per stream (bit): parity of its next weights, of its last output's reading
-      uint32_t nq = 0;
-      bool run = true;
-      auto next_slot = [&](int& i, uint32_t& par) {
-        i = slot;
-        par = fill;
-        if (++slot == NS) {
-          slot = 0;
-          fill ^= 1;
-        }
-      };
-      auto scores = [&](int s, int k) {
-        fence_after();
-        issue_scores<HD>(el, tmem + kColS + s * 128, q0 + (NQ == 1 ? 0 : s) * kTileBytes, ring0 + k * kTileBytes);
-        mma_commit(el, &s_full[s]);
-      };
-      // O_s += P_s V with the V of slot v; the first wait takes two tiles with it
-      auto values = [&](int s, int v, bool fresh, uint32_t bar1, uint32_t par1, uint32_t bar2, uint32_t par2) {
-        const uint32_t s_col = tmem + kColS + s * 128, o_col = tmem + kColO + s * 128, part = part0 + 16 * s;
-        const uint32_t par = parts >> s & 1u, vb = ring0 + v * kTileBytes;
-        run = run && mbar_wait3_warp(part, par, bar1, par1, bar2, par2, vabort);
-        if (!run) return;
-        fence_after();
-        issue_values<HD>(el, o_col, s_col, vb, 0, fresh);
-        run = mbar_wait_warp(part + 8, par, vabort);
-        if (!run) return;
-        fence_after();
-        issue_values<HD>(el, o_col, s_col, vb, 1, false);
-        parts ^= 1u << s;
-      };
-      while (run && walk.next(g)) {
-        int n[2];
-        counts(g, n);
-        const int nt = g.t1 - g.t0;
-        int k, v, ahead = 0;
-        uint32_t kp, vp, ap = 0;
-        next_slot(k, kp);
-        run = mbar_wait3_warp(su32(q_full), nq, full0 + 8 * k, kp, full0 + 8 * k, kp, vabort);
-        nq ^= 1;
-        if (!run) break;
-        scores(0, k);
-        if (NQ == 1) {
-          // tiles i and i + 1 are on the streams' way; ring order K0 V0 K1 V1 ...
-          mma_commit(el, &slot_empty[k]);
-          next_slot(v, vp);
-          int v1 = v;
-          uint32_t v1p = vp;
-          if (nt > 1) {
-            next_slot(k, kp);
-            run = mbar_wait_warp(full0 + 8 * k, kp, vabort);
-            if (!run) break;
-            scores(1, k);
-            mma_commit(el, &slot_empty[k]);
-            next_slot(v1, v1p);
+              tma_load_2d(el, dst + h * kHalfBytes + p * bs * 128, map, h * 64, y[p], bar);
           }
-          if (nt <= 2) mma_commit(el, q_empty);
-          // both outputs of the segment before have been read
-          run = mbar_wait_warp(&o_empty[0], outs & 1u, vabort);
-#pragma unroll 1
-          for (int i = 0; run && i < nt; ++i) {
-            const int s = i & 1;
-            const bool more = i + 2 < nt;
-            const uint32_t vbar = full0 + 8 * v;
-            if (more) {
-              next_slot(ahead, ap);
-            }
-            values(s, v, i < 2, vbar, vp, more ? full0 + 8 * ahead : vbar, more ? ap : vp);
-            if (!run) break;
-            mma_commit(el, &slot_empty[v]);
-            v = v1;
-            vp = v1p;
-            if (more) {
-              scores(s, ahead);
-              mma_commit(el, &slot_empty[ahead]);
-              if (i + 3 == nt) mma_commit(el, q_empty);
-              next_slot(v1, v1p);
-            } else {
-              mma_commit(el, &o_full[s]);
-            }
-          }
-          outs ^= 1u;
-        } else {
-          if (n[1] > 0) scores(1, k);
-          mma_commit(el, &slot_empty[k]);
-          if (nt == 1) mma_commit(el, q_empty);
-#pragma unroll 1
-          for (int i = 0; run && i < nt; ++i) {
-            next_slot(v, vp);
-            const bool more = i + 1 < nt;
-            if (more) next_slot(k, kp);
-            const uint32_t vbar = full0 + 8 * v, kbar = more ? full0 + 8 * k : vbar;
-            if (!more) kp = vp;
-            auto stream = [&](int s) {
-              if (i == 0) run = run && mbar_wait_warp(&o_empty[s], outs >> s & 1u, vabort);
-              values(s, v, i == 0, vbar, vp, kbar, kp);
-              if (!run) return;
-              if (more) {
-                scores(s, k);
-              } else {
-                mma_commit(el, &o_full[s]);
-                outs ^= 1u << s;
-              }
-            };
-            stream(0);
-            if (run && n[1] > 0) stream(1);
-            if (!run) break;
-            mma_commit(el, &slot_empty[v]);
-            if (more) mma_commit(el, &slot_empty[k]);
-            if (i + 2 == nt) mma_commit(el, q_empty);
+          if (guarded) ++gd;
+          slot += 2;
+          if (slot >= NS) {
+            slot -= NS;
+            fill ^= 1;
           }
         }
       }
-      mma_commit(el, final_bar);
+    } else if (warp == kHelp + 3) {
+      // -------------------------------------------------------------- queries
+      if (lane == 0) {
+        int n = 0;
+#pragma unroll 1
+        while (walk.next(g)) {
+          if (!mbar_wait(q_empty, (n & 1) ^ 1, vabort)) break;
+          // (the segment kSegs before has been written out: the one before this
+          // has made its last scores, which came after its own first product,
+          // and that after the reading of the output before it)
+          Seg& x = segs[n % kSegs];
+          const int node0 = g.block * a.block_nodes;
+          x.q0 = g.r.n0 + node0;
+          x.nodes = min(a.block_nodes, g.r.nodes - node0);
+          x.hk = g.hk;
+          x.slot = g.r.slot;
+          x.ctx = g.r.ctx;
+          x.row_nodes = g.r.nodes;
+          x.t0 = g.t0;
+          x.t1 = g.t1;
+          x.tiles = g.tiles;
+          x.first = g.first;
+          x.g0 = guard_from(g);
+          last_bar[NS] = n & 1;
+          ++n;
+          const int tiles = NQ == 2 && x.nodes > tpt ? 2 : 1;
+          mbar_expect_tx(q_full, tiles * kHalves * tpt * group * 128);
+#pragma unroll 1
+          for (int i = 0; i < tiles * kHalves; ++i)
+            tma_load_3d(q_s + i * kHalfBytes, &tmq, (i % kHalves) * 64, g.hk * group,
+                        g.r.n0 + node0 + i / kHalves * tpt, q_full);
+        }
+      }
     } else {
       // -------------------------------------------------------------- guard
-      int c = 0, gd = 0, items = 0;
-      bool run = true;
+      int gd = 0, tiles = 0, items = 0;
+#pragma unroll 1
       while (run && walk.next(g)) {
-        const int nt = g.t1 - g.t0, g0 = guard_from(g);
+        const int g0 = guard_from(g);
         int marks = 0;
+#pragma unroll 1
         for (int t = g0; t < g.t1; ++t, ++gd) {
-          if (!mbar_wait_warp(&guard_full[gd % kGuards], (gd / kGuards) & 1, vabort)) {
-            run = false;
-            break;
-          }
-          const int s = (c + v_at(t - g.t0)) % NS;
+          run = mbar_wait_warp(&guard_full[gd % kGuards], (gd / kGuards) & 1, vabort);
+          if (!run) break;
+          const int s = (2 * (tiles + t - g.t0) + 1) % NS;
           if (tile::clear_nonfinite(reinterpret_cast<uint4*>(ring + s * kTileBytes), kTileBytes / 16))
             marks |= 1 << min(t - g0, 31);
           if (lane == 0) {
@@ -574,153 +656,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_arrive(&slot_full[s]);
           }
         }
-        c += 2 * nt;
+        tiles += g.t1 - g.t0;
         ++items;
       }
     }
-  } else {
-    // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int s = warp >> 2, q4 = warp & 3, r = tid & 127;
-    const uint32_t lane_base = tmem + ((uint32_t)(32 * q4) << 16);
-    const int rt = r / group, rg = r - rt * group;
-    int nt_done = 0, items = 0, no[2] = {0, 0};
-    Cut cut{-1, 0, 0, 0};
-    bool run = true;
-    while (run && walk.next(g)) {
-      int n[2];
-      counts(g, n);
-      const int item = items++;
-      if (NQ == 2 && n[s] == 0) continue;
-      const int node = g.block * a.block_nodes + (NQ == 2 ? s * tpt : 0) + rt;
-      const bool valid = rt < tpt && node < g.r.nodes;
-      const uint32_t valid_rows = __ballot_sync(0xffffffffu, valid);
-      const int g0 = guard_from(g);
-      const uint32_t* mask = reinterpret_cast<const uint32_t*>(a.masks + (int64_t)(g.r.n0 + (valid ? node : 0)) * a.words);
-      // the first word of the mask (all of it, up to 64 nodes) on its way early
-      const uint2 head = __ldg(reinterpret_cast<const uint2*>(mask));
-      auto bits = [&](int key0) {
-        return visible32([&](int i) { return i == 0 ? head.x : i == 1 ? head.y : __ldg(mask + i); }, a.words, g.r, key0);
-      };
-      tile::RowState row;
-      row.reset();
-      for (int j = 0; j < n[s]; ++j, ++nt_done) {
-        const int t = g.t0 + (NQ == 1 ? 2 * j + s : j);
-        const bool masked = t >= g0;
-        uint32_t vis[4] = {0u, 0u, 0u, 0u};
-        if (masked && valid) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) vis[x] = bits(t * 128 + 32 * x);
-        }
-        if (!mbar_wait_warp(&s_full[s], nt_done & 1, vabort)) {
-          run = false;
-          break;
-        }
-        fence_after();
-        if (!valid_rows) {
-          if (lane == 0) {
-            mbar_arrive(&p_half[2 * s]);
-            mbar_arrive(&p_half[2 * s + 1]);
-          }
-          continue;
-        }
-        tile::softmax_tile<HD>(lane_base, kColS + s * 128, kColO + s * 128, a.scale_log2, j == 0, masked, vis, row,
-                               &p_half[2 * s], &p_half[2 * s + 1]);
-      }
-      if (!run) break;
-      float M = row.m, L = row.l, f0 = 1.f, f1 = 0.f;
-      if (NQ == 1) {
-        // the other stream's statistics of the same row
-        float* x = ml + (item & 1) * 512;
-        *reinterpret_cast<float2*>(x + s * 256 + 2 * r) = make_float2(row.m, row.l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&x_bar[q4]);
-        const uint32_t full0 = su32(&o_full[0]);
-        run = mbar_wait3_warp(su32(&x_bar[q4]), item & 1, full0, no[0] & 1, n[1] > 0 ? full0 + 8 : full0,
-                              (n[1] > 0 ? no[1] : no[0]) & 1, vabort);
-        ++no[0];
-        no[1] += n[1] > 0 ? 1 : 0;
-        if (!run) break;
-        const float2 s0 = *reinterpret_cast<const float2*>(x + 2 * r);
-        const float2 s1 = *reinterpret_cast<const float2*>(x + 256 + 2 * r);
-        M = fmaxf(s0.x, s1.x);
-        const float ms = M == -INFINITY ? 0.f : M;
-        f0 = ex2(s0.x - ms);
-        f1 = n[1] > 0 ? ex2(s1.x - ms) : 0.f;
-        L = s0.y * f0 + s1.y * f1;  // a sum is finite or the NaN of a score
-      } else {
-        run = mbar_wait_warp(&o_full[s], no[0] & 1, vabort);
-        ++no[0];
-        if (!run) break;
-      }
-      fence_after();
-      const int marks = g0 < g.t1 ? poison[item % kGuards] : 0;
-      const bool whole = g.t0 == 0 && g.t1 == g.tiles;
-      const float inv = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
-      float* mine = part(a, blockIdx.x, g.t0 == 0);
-      const int prow = (NQ == 2 ? s * 128 : 0) + r;
-      if (g.t0 == 0 && !whole)
-        cut = Cut{owner(span, g.first + g.tiles - 1), g.r.n0 + g.block * a.block_nodes,
-                  min(a.block_nodes, g.r.nodes - g.block * a.block_nodes), g.hk};
-      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + (int64_t)(g.r.n0 + node) * a.o_tok +
-                           (int64_t)(g.hk * group + rg) * a.o_head + (NQ == 1 ? s * HDS : 0);
-#pragma unroll 1
-      for (int h = 0; h < HDS / 32; ++h) {
-        const int col = (NQ == 1 ? s * HDS : 0) + 32 * h;
-        uint32_t u[32];
-        float* o = reinterpret_cast<float*>(u);
-        if (NQ == 1) {
-          tmem_ld32(lane_base + kColO + col, u);
-          tmem_wait_ld();
-#pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = f0 == 0.f ? 0.f : o[x] * f0;
-          if (n[1] > 0) {
-            uint32_t u1[32];
-            tmem_ld32(lane_base + kColO + 128 + col, u1);
-            tmem_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] += f1 == 0.f ? 0.f : __uint_as_float(u1[x]) * f1;
-          }
-        } else {
-          tmem_ld32(lane_base + kColO + s * 128 + col, u);
-          tmem_wait_ld();
-        }
-        if (h == HDS / 32 - 1) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_empty[NQ == 1 ? 0 : s]);
-        }
-        if (marks && valid) {
-          const int first = max(g0 * 128, 0), keys = min(g.r.ctx + g.r.nodes, g.t1 * 128);
-#pragma unroll 1
-          for (int key = first; key < keys; ++key) {
-            if (!(marks >> min((key >> 7) - g0, 31) & 1) || !(bits(key & ~31) >> (key & 31) & 1u)) continue;
-            const int bi = key / a.block_size;
-            if (g.r.slot < 0 || bi >= min(a.nblocks[g.r.slot], a.max_blocks)) continue;
-            const int blk = a.block_table[(int64_t)g.r.slot * a.max_blocks + bi];
-            if (blk < 0 || blk >= a.num_blocks) continue;
-            const __nv_bfloat16* v =
-                reinterpret_cast<const __nv_bfloat16*>(a.v_pool) +
-                (((int64_t)blk * a.rows.kv_heads + g.hk) * a.block_size + key % a.block_size) * HD + col;
-#pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              const float y = __bfloat162float(v[x]);
-              if (!isfinite(y)) o[x] += y;
-            }
-          }
-        }
-        if (valid && whole) {
-          tile::store_row32(dst + 32 * h, o, inv, a.out_vec);
-        } else if (valid) {
-          float4* p = reinterpret_cast<float4*>(part_row(a, mine, prow) + col);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) __stcg(p + x, make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]));
-        }
-      }
-      if (!whole && valid && (NQ == 2 || s == 0))
-        __stcg(reinterpret_cast<float2*>(part_stats(a, mine, prow)), make_float2(M, L));
-    }
-    if (tid == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(cut.last, cut.node0, cut.nodes, cut.hk);
   }
 
   __syncthreads();
@@ -733,11 +672,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     if (last_bar[NS] >= 0) mbar_drain(q_full, last_bar[NS]);
   }
-  if (warp == 9) {
+  if (warp == kHelp + 1) {
     if (lane == 0) mbar_drain(final_bar, 0);
     __syncwarp();
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem));
   }
 }
 
@@ -762,10 +701,10 @@ template <int HD, int NQ>
 int launch_tc(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
   auto kern = tree_tc_kernel<HD, NQ>;
   constexpr size_t smem = tc_smem_bytes<HD, NQ>();
-  static_assert(smem + 320 <= 227 * 1024, "shared memory");
+  static_assert(smem + 640 <= 227 * 1024, "shared memory");
   static const cudaError_t opt = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (opt != cudaSuccess) return (int)opt;
-  const int tpt = 128 / a.rows.group;
+  const int tpt = 128 / a.rows.group, ctas = NQ == 1 ? 2 * kNumSMs : kNumSMs;
   a.block_nodes = NQ * tpt;
   CUtensorMap mq, mk, mv;
   int rc = g_q_maps.get(Map3Key{reinterpret_cast<uint64_t>(a.q), (uint64_t)HD, (uint64_t)q_heads,
@@ -778,9 +717,9 @@ int launch_tc(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
   if (rc) return rc;
   a.part_rows = 128 * NQ;
   if (!countable(a.rows, 128, a.block_nodes)) return PSE_EINVAL;
-  const cudaError_t e = launch_pdl(kern, dim3(kNumSMs), dim3(kTcThreads), smem, s, mq, mk, mv, a);
+  const cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(n_threads<NQ>()), smem, s, mq, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
-  return launch_join<__nv_bfloat16>(a, kNumSMs, max_nodes, tpt * a.rows.group, 128, s);
+  return launch_join<__nv_bfloat16>(a, ctas, max_nodes, tpt * a.rows.group, 128, s);
 }
 
 template <int HD>
@@ -831,7 +770,7 @@ extern "C" int pse_tree_masks(const int32_t* parents, const int32_t* node_off, i
 extern "C" size_t pse_token_tree_workspace(int32_t head_dim) {
   if (head_dim <= 0) return 0;
   // two partial results per CTA: of 64 rows on the CUDA cores, of 256 on the tensor cores
-  const size_t simt = (size_t)tree::kMaxCtas * 64, tc = (size_t)kNumSMs * 256;
+  const size_t simt = (size_t)tree::kMaxWorkers * 64, tc = (size_t)kNumSMs * 256;
   return tree::kCutBytes + (head_dim <= 128 && tc > simt ? tc : simt) * 2 * (head_dim + 2) * 4;
 }
 

@@ -1,16 +1,17 @@
-// How the work of one token-tree attention call is split over the CTAs.
+// How the work of one token-tree attention call is split over its workers, the
+// CTAs.
 //
 // Row i (a request) has nodes_i queries per head over ctx_i + nodes_i keys.  Its
 // items are (query block, K/V head), each a run of ceil(keys / tile) key tiles.
-// The tiles of all items of all rows, in order, form one line of T tiles; CTA
-// c of G takes the tiles [c T / G, (c + 1) T / G), so every CTA has the same
-// number of tiles (within one) whatever the lengths are, and nothing about
-// them has to be known on the host.  An item whose tiles all fall to one CTA
-// is finished there.  An item cut by CTA boundaries leaves one partial result
-// per CTA (maximum, sum and unnormalised output) in the workspace, which a
-// second, small kernel joins in the order of the CTAs.  (Joining by the last CTA
-// to arrive saves that launch but leaves the rows of an item to one warp each
-// 32, serially: 158 us instead of %JOIN% at 64 requests of 128 to 4096 tokens.)
+// The tiles of all items of all rows, in order, form one line of T tiles; worker
+// c of G takes T / G of them (the first T mod G one more), so every worker has
+// the same number of tiles whatever the lengths are, and nothing about them has
+// to be known on the host.  An item whose tiles all fall to one worker is
+// finished there.  An item cut by the workers' bounds leaves one partial result
+// per worker (maximum, sum and unnormalised output) in the workspace, which a
+// second, small kernel joins in the order of the workers.  (Joining by the last
+// of them to arrive saves that launch but leaves an item's rows to one CTA:
+// 158 us instead of 95 at 64 requests of 128 to 4096 tokens, all else equal.)
 #pragma once
 
 #include "common.cuh"
@@ -58,10 +59,12 @@ __device__ __forceinline__ int key_tiles(const Row& r) {
 
 // All counts of tiles fit 31 bits (the entry point checks the largest that the
 // block table allows): 64-bit divisions took longer than the loads of a tile.
+struct Split {
+  int per, extra;    // tiles per worker; the first `extra` workers have one more
+  int workers;       // workers that have tiles
+};
 struct Span {
-  int begin, end;    // this CTA's tiles
-  int per, extra;    // tiles per CTA; the first `extra` CTAs have one more
-  int ctas;          // CTAs that have tiles
+  int begin, end;    // a worker's tiles
   int row, off;      // row of the first tile, and its offset within the row
 };
 
@@ -70,12 +73,14 @@ __device__ __forceinline__ int row_weight(const Rows& a, const Row& r, int block
   return r.nodes > 0 ? key_tiles<TILE>(r) * q_blocks(a, r, block_nodes) * a.kv_heads : 0;
 }
 
-// All threads of the CTA; `tmp` holds 36 ints of shared memory.
+// The span of this CTA, worker blockIdx.x of gridDim.x.  All threads of the CTA;
+// `tmp` holds 36 ints of shared memory.
 template <int TILE>
-__device__ Span my_span(const Rows& a, int block_nodes, int* tmp) {
+__device__ Split my_span(const Rows& a, int block_nodes, int* tmp, Span& x) {
   const int per = (a.rows + blockDim.x - 1) / blockDim.x;
   const int lo = min(a.rows, (int)threadIdx.x * per), hi = min(a.rows, lo + per);
   int mine = 0, first = 0;
+#pragma unroll 1
   for (int i = lo; i < hi; ++i) {
     const int w = row_weight<TILE>(a, read_row(a, i), block_nodes);
     if (i == lo) first = w;
@@ -87,22 +92,24 @@ __device__ Span my_span(const Rows& a, int block_nodes, int* tmp) {
   if (lane == 31) tmp[warp] = inc;
   __syncthreads();
   int before = inc - mine, total = 0;
+#pragma unroll 1
   for (int w = 0; w < nw; ++w) {
-    const int x = tmp[w];
-    before += w < warp ? x : 0;
-    total += x;
+    const int y = tmp[w];
+    before += w < warp ? y : 0;
+    total += y;
   }
-  Span s;
-  s.ctas = min((int)gridDim.x, total);
-  s.per = s.ctas > 0 ? total / s.ctas : 0;
-  s.extra = total - s.per * s.ctas;
+  Split s;
+  s.workers = min((int)gridDim.x, total);
+  s.per = s.workers > 0 ? total / s.workers : 0;
+  s.extra = total - s.per * s.workers;
   const int c = blockIdx.x;
-  s.begin = s.end = s.row = s.off = 0;
-  if (c < s.ctas) {
-    s.begin = s.per * c + min(c, s.extra);
-    s.end = s.begin + s.per + (c < s.extra ? 1 : 0);
-    if (s.begin >= before && s.begin < before + mine) {
-      int at = s.begin - before, i = lo, w = first;
+  x.begin = x.end = x.row = x.off = 0;
+  if (c < s.workers) {
+    x.begin = s.per * c + min(c, s.extra);
+    x.end = x.begin + s.per + (c < s.extra ? 1 : 0);
+    if (x.begin >= before && x.begin < before + mine) {
+      int at = x.begin - before, i = lo, w = first;
+#pragma unroll 1
       while (at >= w) {
         at -= w;
         w = row_weight<TILE>(a, read_row(a, ++i), block_nodes);
@@ -112,20 +119,20 @@ __device__ Span my_span(const Rows& a, int block_nodes, int* tmp) {
     }
   }
   __syncthreads();
-  if (c < s.ctas) {
-    s.row = tmp[32];
-    s.off = tmp[33];
+  if (c < s.workers) {
+    x.row = tmp[32];
+    x.off = tmp[33];
   }
   return s;
 }
 
-// The CTA that has tile x.
-__device__ __forceinline__ int owner(const Span& s, int x) {
+// The worker that has tile x.
+__device__ __forceinline__ int owner(const Split& s, int x) {
   const int cut = s.extra * (s.per + 1);
   return x < cut ? x / (s.per + 1) : s.extra + (x - cut) / s.per;
 }
 
-// One run of tiles of one item, within one CTA.
+// One run of tiles of one item, within one worker.
 struct Segment {
   int hk, block;          // the item: K/V head and query block
   Row r;
@@ -139,27 +146,33 @@ inline bool countable(const Rows& a, int tile, int block_nodes) {
   return (double)tiles * (double)blocks * a.kv_heads * a.rows < 2147483647.0;
 }
 
-// Walks a CTA's segments.
+// Walks a worker's segments.
 template <int TILE>
 struct Walk {
-  const Rows& a;
+  const Rows* rows;
   int block_nodes, at, end, row, off, w, nt, nb;  // next tile on the line, ...; the row's weight, tiles, blocks
   Row r;
-  __device__ Walk(const Rows& rows, const Span& span, int bn)
-      : a(rows), block_nodes(bn), at(span.begin), end(span.end), row(span.row), off(span.off) {
+  __device__ __forceinline__ void start(const Rows& a, const Span& span, int bn) {
+    rows = &a;
+    block_nodes = bn;
+    at = span.begin;
+    end = span.end;
+    row = span.row;
+    off = span.off;
     if (at < end) load();
   }
   __device__ __forceinline__ void load() {
-    r = read_row(a, row);
+    r = read_row(*rows, row);
     nt = key_tiles<TILE>(r);
-    nb = q_blocks(a, r, block_nodes);
-    w = nt * nb * a.kv_heads;
+    nb = q_blocks(*rows, r, block_nodes);
+    w = nt * nb * rows->kv_heads;
   }
   __device__ bool next(Segment& g) {
     if (at >= end) return false;
+#pragma unroll 1
     while (off >= w) {
       off -= w;
-      if (++row >= a.rows) return false;
+      if (++row >= rows->rows) return false;
       load();
     }
     const int item = off / nt;
@@ -181,18 +194,18 @@ struct Walk {
 // below the context, then the nodes its mask names; word(i): the mask's i-th 32
 // bits (i < 2 words).
 template <typename F>
-__device__ __forceinline__ uint32_t visible32(F word, int words, const Row& r, int key0) {
-  if (r.slot < 0) return 0u;
-  const int d = key0 - r.ctx;
+__device__ __forceinline__ uint32_t visible32(F word, int words, int slot, int ctx, int nodes, int key0) {
+  if (slot < 0) return 0u;
+  const int d = key0 - ctx;
   if (d <= -32) return 0xffffffffu;
   uint32_t bits = d < 0 ? (1u << -d) - 1u : 0u;
   // node bits [max(d, 0), d + 32) of the mask, nodes past the tree never
   const int n0 = max(d, 0), sh = n0 - d;
-  if (n0 < r.nodes) {
+  if (n0 < nodes) {
     const int w = n0 >> 5, b = n0 & 31, nw = 2 * words;
     const uint32_t lo = w < nw ? word(w) : 0u, up = w + 1 < nw ? word(w + 1) : 0u;
     uint32_t x = __funnelshift_r(lo, up, b);
-    const int left = r.nodes - n0;
+    const int left = nodes - n0;
     if (left < 32) x &= (1u << left) - 1u;
     bits |= x << sh;
   }
