@@ -60,61 +60,107 @@ struct Cut {
   int hk;
 };
 
-// A warp per row of a cut item, lanes over the columns: the parts are summed in
-// the order of their workers.
+// A warp per row of the cut items, lanes over the columns: the parts are summed
+// in the order of their workers.  Every block reads all cuts and numbers their
+// rows, so the rows are spread over the whole GPU whatever was cut where.  (A
+// block per cut and row slice instead, most of them idle, took 28 us where this
+// takes 9, two trees of 64 nodes with 8192 tokens each.)
+constexpr int kJoinThreads = 512;
+
 template <typename T, int PER>
-__global__ void join_kernel(const Args a, int tile_rows, int tile_pitch) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, int workers, int tile_rows, int tile_pitch) {
+  __shared__ int scan_tmp[33];
+  __shared__ int first_row[kJoinThreads];  // rows of the cuts before
+  __shared__ int4 cuts[kJoinThreads];
   pdl_wait();
-  const int4 x = *reinterpret_cast<const int4*>(a.cuts + blockIdx.x);
-  const int c1 = blockIdx.x, c2 = x.x, node0 = x.y, hk = x.w, group = a.rows.group, hd = a.hd;
-  const int row = blockIdx.y * (blockDim.x / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (c2 < 0 || row >= x.z * group) return;
-  const int r = row / tile_rows * tile_pitch + row % tile_rows;
-  float M = -INFINITY;
-  for (int c = c1 + lane; c <= c2; c += 32) M = fmaxf(M, part_stats(a, part(a, c, c == c1), r)[0]);
-  M = warp_max(M);
-  const float ms = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc[PER];
+  const int tid = threadIdx.x, lane = tid & 31, group = a.rows.group, hd = a.hd;
+  int4 mine = make_int4(-1, 0, 0, 0);
+  if (tid < workers) mine = __ldcg(reinterpret_cast<const int4*>(a.cuts + tid));
+  int total;
+  const int before = block_exclusive_scan(mine.x >= 0 ? mine.z * group : 0, scan_tmp, &total);
+  first_row[tid] = before;
+  cuts[tid] = mine;
+  __syncthreads();
+  const int warps = gridDim.x * (kJoinThreads / 32);
+#pragma unroll 1
+  for (int task = blockIdx.x * (kJoinThreads / 32) + (tid >> 5); task < total; task += warps) {
+    // the last cut whose rows begin at or before the task (cuts without rows share
+    // their successor's beginning)
+    int c1 = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-  for (int c0 = c1; c0 <= c2; c0 += 32) {
-    const int n = min(32, c2 + 1 - c0);
-    float f = 0.f, l = 0.f;
-    if (lane < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(part_stats(a, part(a, c0 + lane, c0 + lane == c1), r));
-      f = exp2f(ml.x - ms);
-      l = ml.y * f;  // a sum is finite or the NaN of a score
-    }
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      L += __shfl_sync(0xffffffffu, l, i);
-      const float* p = part_row(a, part(a, c0 + i, c0 + i == c1), r);
+    for (int step = kJoinThreads / 2; step > 0; step >>= 1)
+      if (first_row[c1 + step] <= task) c1 += step;
+    const int4 cut = cuts[c1];
+    const int c2 = cut.x, row = task - first_row[c1];
+    const int r = row / tile_rows * tile_pitch + row % tile_rows;
+    // worker c1 holds the item's beginning in its second block, the others theirs
+    // in their first
+    const int64_t pitch = 2ll * a.part_rows * (hd + 2);
+    const float* base = a.parts + c1 * pitch + (int64_t)a.part_rows * (hd + 2);
+    auto block = [&](int i) -> const float* {  // of worker c1 + i
+      return i == 0 ? base : base + i * pitch - (int64_t)a.part_rows * (hd + 2);
+    };
+    const int64_t stats = (int64_t)a.part_rows * hd + 2 * r;
+    const int n = c2 - c1 + 1;
+    // four parts' values on their way before the statistics that weigh them
+    float v[4][PER];
+    auto load = [&](int i0) {
 #pragma unroll
-      for (int y = 0; y < PER; ++y) {
-        const int d = lane + 32 * y;
-        if (d < hd) acc[y] += fi == 0.f ? 0.f : p[d] * fi;
+      for (int i = 0; i < 4; ++i) {
+        const float* p = block(min(i0 + i, n - 1)) + (int64_t)r * hd;
+#pragma unroll
+        for (int y = 0; y < PER; ++y) v[i][y] = lane + 32 * y < hd ? __ldcg(p + lane + 32 * y) : 0.f;
+      }
+    };
+    load(0);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < n) ml = __ldcg(reinterpret_cast<const float2*>(block(lane) + stats));
+    float M = ml.x;
+#pragma unroll 1
+    for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, __ldcg(block(i) + stats));
+    M = warp_max(M);
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 4) {
+      if (i0 > 0) {
+        load(i0);
+        if ((i0 & 31) == 0) {
+          ml = make_float2(-INFINITY, 0.f);
+          if (i0 + lane < n) ml = __ldcg(reinterpret_cast<const float2*>(block(i0 + lane) + stats));
+        }
+      }
+      const float f = exp2f(ml.x - ms), l = ml.y * f;  // a sum is finite or the NaN of a score
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i0 + i >= n) break;
+        const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
+        L += __shfl_sync(0xffffffffu, l, (i0 + i) & 31);
+#pragma unroll
+        for (int y = 0; y < PER; ++y) acc[y] += fi == 0.f ? 0.f : v[i][y] * fi;
       }
     }
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(node0 + row / group) * a.o_tok +
-           (int64_t)(hk * group + row % group) * a.o_head;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(cut.y + row / group) * a.o_tok +
+             (int64_t)(cut.w * group + row % group) * a.o_head;
 #pragma unroll
-  for (int y = 0; y < PER; ++y) {
-    const int d = lane + 32 * y;
-    if (d < hd) dst[d] = from_f32<T>(acc[y] * inv);
+    for (int y = 0; y < PER; ++y) {
+      const int d = lane + 32 * y;
+      if (d < hd) dst[d] = from_f32<T>(acc[y] * inv);
+    }
   }
 }
 
 template <typename T>
-int launch_join(const Args& a, int workers, int max_nodes, int tile_rows, int tile_pitch, cudaStream_t s) {
-  const int rows = (max_nodes < a.block_nodes ? max_nodes : a.block_nodes) * a.rows.group;
-  const int warps = rows < 16 ? rows : 16;
-  const dim3 grid(workers, ceil_div(rows, warps)), block(32 * warps);
-  const cudaError_t e = a.hd <= 64    ? launch_pdl(join_kernel<T, 2>, grid, block, 0, s, a, tile_rows, tile_pitch)
-                        : a.hd <= 128 ? launch_pdl(join_kernel<T, 4>, grid, block, 0, s, a, tile_rows, tile_pitch)
-                                      : launch_pdl(join_kernel<T, 8>, grid, block, 0, s, a, tile_rows, tile_pitch);
+int launch_join(const Args& a, int workers, int tile_rows, int tile_pitch, cudaStream_t s) {
+  static_assert(kMaxWorkers <= kJoinThreads, "a thread per cut");
+  const dim3 grid(3 * kNumSMs), block(kJoinThreads);
+  const cudaError_t e =
+      a.hd <= 64    ? launch_pdl(join_kernel<T, 2>, grid, block, 0, s, a, workers, tile_rows, tile_pitch)
+      : a.hd <= 128 ? launch_pdl(join_kernel<T, 4>, grid, block, 0, s, a, workers, tile_rows, tile_pitch)
+                    : launch_pdl(join_kernel<T, 8>, grid, block, 0, s, a, workers, tile_rows, tile_pitch);
   return e == cudaSuccess ? PSE_OK : (int)e;
 }
 
@@ -245,7 +291,7 @@ int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
   a.part_rows = 16 * rpt;
   if (!countable(a.rows, simt::BK, a.block_nodes)) return PSE_EINVAL;
   const int rc = rpt == 1 ? simt_nc<T, 1>(a, kMaxWorkers, s) : simt_nc<T, 4>(a, kMaxWorkers, s);
-  return rc == PSE_OK ? launch_join<T>(a, kMaxWorkers, max_nodes, a.part_rows, a.part_rows, s) : rc;
+  return rc == PSE_OK ? launch_join<T>(a, kMaxWorkers, a.part_rows, a.part_rows, s) : rc;
 }
 
 // ---------------------------------------------------------------- tensor cores
@@ -262,7 +308,7 @@ int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
 //   0 .. h - 1  the softmax (attention_tile.cuh), a thread per row, and the output
 //   h, h + 4    K, and V pages by TMA into a ring of 128-key slots (a copy takes
 //               its warp some 50 clocks to issue, and a tile of 16-token pages is
-//               16 copies)
+//               16 copies; two streams leave one warp the time for both)
 //   h + 1       the products
 //   h + 2       clears V tiles that hold nodes (or what stands after them) of
 //               infinities and NaN before the product, as in prompt_attention.cu
@@ -274,7 +320,7 @@ constexpr int kHalfBytes = 128 * 128;
 constexpr int kGuards = 8;
 
 template <int NQ>
-__host__ __device__ constexpr int n_threads() { return 32 * (4 * NQ + 5); }
+__host__ __device__ constexpr int n_threads() { return 32 * (4 * NQ + (NQ == 1 ? 5 : 4)); }
 // two CTAs share a multiprocessor's 227 KB when NQ = 1: at head_dim 128 a K and a
 // V tile each, whose loads still pass behind the other tile's softmax
 template <int HD, int NQ>
@@ -361,8 +407,11 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
   auto guard_from = [&](const Segment& x) { return max(x.t0, x.r.slot < 0 ? 0 : x.r.ctx >> 7); };
   bool run = true;
 
+  // (two streams hold a row of scores in registers: the other warps give some up)
+  if (NQ == 2 && warp >= kHelp) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   if (warp < kHelp) {
     // ---------------------------------------------------------------- softmax
+    if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int s = NQ == 1 ? 0 : warp >> 2, r = tid & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const int rt = r / group, rg = r - rt * group;
@@ -408,8 +457,12 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
           }
           continue;
         }
-        tile::softmax_tile_small<HD>(lane_base, s * 128, kColO + s * 128, a.scale_log2, t == t0, masked, vis[0], vis[1],
-                                     vis[2], vis[3], row, su32(&p_half[2 * s]));
+        if (NQ == 1)
+          tile::softmax_tile_small<HD>(lane_base, s * 128, kColO + s * 128, a.scale_log2, t == t0, masked, vis[0], vis[1],
+                                       vis[2], vis[3], row, su32(&p_half[2 * s]));
+        else
+          tile::softmax_tile<HD>(lane_base, s * 128, kColO + s * 128, a.scale_log2, t == t0, masked, vis, row,
+                                 &p_half[2 * s], &p_half[2 * s + 1]);
       }
       if (!run || !mbar_wait_warp(&o_full[s], items & 1, vabort)) break;
       fence_after();
@@ -509,19 +562,20 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
           nt = x.t1 - x.t0;
           left -= nt;
         }
-#pragma unroll 1
-        for (int s = 0; run && s < NQ; ++s) {
+#pragma unroll
+        for (int s = 0; s < NQ; ++s) {
+          if (!run) break;
           const uint32_t s_col = tmem + s * 128, o_col = tmem + kColO + s * 128;
           if (i >= 0) {
             const uint32_t part = part0 + 16 * s, par = parts >> s & 1u;
             // the output of the segment before has been read
             if (i == 0) run = mbar_wait_warp(&o_empty[s], outs >> s & 1u, vabort);
-            // (at two slots the next K waits for this tile's V to leave its own)
-            run = run && mbar_wait3_warp(part, par, vbar, vp, vbar, vp, vabort);
+            run = run && (s == 0 ? mbar_wait3_warp(part, par, vbar, vp, kbar, kp, vabort)
+                                 : mbar_wait_warp(part, par, vabort));
             if (!run) break;
             fence_after();
             issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 0, i == 0);
-            run = mbar_wait3_warp(part + 8, par, kbar, kp, kbar, kp, vabort);
+            run = mbar_wait_warp(part + 8, par, vabort);
             if (!run) break;
             fence_after();
             issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 1, false);
@@ -548,14 +602,14 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
     Walk<128> walk;
     walk.start(a.rows, span, a.block_nodes);
     Segment g;
-    if (warp == kHelp || warp == kHelp + 4) {
+    if (warp == kHelp || (NQ == 1 && warp == kHelp + 4)) {
       // -------------------------------------------------------------- pages
-      const bool is_v = warp != kHelp;
+      // NQ = 1: this warp's K or V tiles, every second slot; NQ = 2: both in turn
+      const int kv0 = warp == kHelp ? 0 : 1, kv1 = NQ == 1 ? kv0 : 1;
       const int bs = a.block_size, ppt = 128 / bs, tpc = 32 / ppt, oob = a.num_blocks * a.rows.kv_heads * bs;
       const uint32_t el = elect_one();
       const uint32_t empty0 = su32(slot_empty), full0 = su32(slot_full), guard0 = su32(guard_full), ring0 = su32(ring);
-      const CUtensorMap* map = is_v ? &tmv : &tmk;
-      int gd = 0, slot = is_v ? 1 : 0;
+      int gd = 0, slot = kv0;
       uint32_t fill = 0;
 #pragma unroll 1
       while (run && walk.next(g)) {
@@ -571,36 +625,41 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
         };
         int cur = page(lane), nxt = page(32 + lane);
 #pragma unroll 1
-        for (int t = g.t0; t < g.t1; ++t) {
+        for (int t = g.t0; run && t < g.t1; ++t) {
           const int i = t - g.t0, src = (i & (tpc - 1)) * ppt;
           if (i > 0 && src == 0) {
             cur = nxt;
             nxt = page(32 * (i / tpc + 1) + lane);
           }
-          run = mbar_wait_warp(empty0 + 8 * slot, fill ^ 1, vabort);
-          if (!run) break;
-          const bool guarded = is_v && t >= g0;
-          const uint32_t bar = guarded ? guard0 + 8 * (gd % kGuards) : full0 + 8 * slot;
-          if (el) {
-            last_bar[slot] = guarded ? (NS + gd % kGuards) * 2 + ((gd / kGuards) & 1) : slot * 2 + (int)fill;
-            mbar_expect_tx(bar, kTileBytes);
-          }
           int y[8];
 #pragma unroll
           for (int p = 0; p < 8; ++p) y[p] = __shfl_sync(0xffffffffu, cur, (src + p) & 31);
-          const uint32_t dst = ring0 + slot * kTileBytes;
+#pragma unroll 1
+          for (int kv = kv0; kv <= kv1; ++kv) {
+            run = mbar_wait_warp(empty0 + 8 * slot, fill ^ 1, vabort);
+            if (!run) break;
+            const bool guarded = kv == 1 && t >= g0;
+            const uint32_t bar = guarded ? guard0 + 8 * (gd % kGuards) : full0 + 8 * slot;
+            if (el) {
+              last_bar[slot] = guarded ? (NS + gd % kGuards) * 2 + ((gd / kGuards) & 1) : slot * 2 + (int)fill;
+              mbar_expect_tx(bar, kTileBytes);
+            }
+            __syncwarp();
+            const uint32_t dst = ring0 + slot * kTileBytes;
+            const CUtensorMap* map = kv ? &tmv : &tmk;
 #pragma unroll
-          for (int p = 0; p < 8; ++p) {
-            if (p >= ppt) break;
+            for (int p = 0; p < 8; ++p) {
+              if (p >= ppt) break;
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-              tma_load_2d(el, dst + h * kHalfBytes + p * bs * 128, map, h * 64, y[p], bar);
-          }
-          if (guarded) ++gd;
-          slot += 2;
-          if (slot >= NS) {
-            slot -= NS;
-            fill ^= 1;
+              for (int h = 0; h < kHalves; ++h)
+                tma_load_2d(el, dst + h * kHalfBytes + p * bs * 128, map, h * 64, y[p], bar);
+            }
+            if (guarded) ++gd;
+            slot += NQ == 1 ? 2 : 1;
+            if (slot >= NS) {
+              slot -= NS;
+              fill ^= 1;
+            }
           }
         }
       }
@@ -719,7 +778,7 @@ int launch_tc(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
   if (!countable(a.rows, 128, a.block_nodes)) return PSE_EINVAL;
   const cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(n_threads<NQ>()), smem, s, mq, mk, mv, a);
   if (e != cudaSuccess) return (int)e;
-  return launch_join<__nv_bfloat16>(a, ctas, max_nodes, tpt * a.rows.group, 128, s);
+  return launch_join<__nv_bfloat16>(a, ctas, tpt * a.rows.group, 128, s);
 }
 
 template <int HD>
