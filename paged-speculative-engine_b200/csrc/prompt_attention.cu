@@ -45,10 +45,12 @@ __global__ void __launch_bounds__(simt::kThreads) prompt_simt_kernel(const Args 
   const int tok0 = it.x, len = it.y, hk = it.w;
   // an item that the tensors do not hold is skipped (a plan made for others)
   if (tok0 < 0 || len < 0 || it.z < 0 || (int64_t)tok0 + len > a.tokens || hk < 0 || hk >= a.kv_heads) return;
-  const int64_t r0 = (int64_t)it.z * a.group + (blockIdx.x % subs) * 64;
-  const int64_t r_end = (int64_t)min(len, it.z + 2 * tile_tokens(a.group)) * a.group;
-  const int nr = (int)min((int64_t)64, r_end - r0);
+  // rows (token, group head) of the item, token-major, from r0; token t of the
+  // prompt's is it.z + row / group
+  const int r0 = (int)(blockIdx.x % subs) * 64;
+  const int nr = min(64, min(len - it.z, 2 * tile_tokens(a.group)) * a.group - r0);
   if (nr <= 0) return;
+  const int first = it.z + r0 / a.group, last = it.z + (r0 + nr - 1) / a.group;  // its tokens
   simt::Tile<4, NC> t;
   t.init(smem, a.hd);
   t.reset();
@@ -58,27 +60,32 @@ __global__ void __launch_bounds__(simt::kThreads) prompt_simt_kernel(const Args 
   const T* q = reinterpret_cast<const T*>(a.q);
   const T* k = reinterpret_cast<const T*>(a.k) + hk * a.k_head;
   const T* v = reinterpret_cast<const T*>(a.v) + hk * a.v_head;
-  t.template fill<T>(
-      t.q, 64,
+  t.template fill_q<T>(
       [&](int r) -> const T* {
         if (r >= nr) return nullptr;
-        const int64_t rr = r0 + r;
-        return q + (tok0 + rr / a.group) * a.q_tok + (hk * a.group + rr % a.group) * a.q_head;
+        const int w = (r0 + r) / a.group;
+        return q + (int64_t)(tok0 + it.z + w) * a.q_tok + (int64_t)(hk * a.group + (r0 + r - w * a.group)) * a.q_head;
       },
       vec(a.q, a.q_tok, a.q_head), a.scale_log2);
-  const int kmax = (int)((r0 + nr - 1) / a.group) + 1;  // keys the last row sees
+  int token[4];  // of this thread's rows
+#pragma unroll
+  for (int i = 0; i < 4; ++i) token[i] = it.z + (r0 + t.ty * 4 + i) / a.group;
   const bool kvec = vec(a.k, a.k_tok, a.k_head), vvec = vec(a.v, a.v_tok, a.v_head);
-  for (int k0 = 0; k0 < kmax; k0 += simt::BK) {
+#pragma unroll 1
+  for (int k0 = 0; k0 <= last; k0 += simt::BK) {
     __syncthreads();
-    t.template fill<T>(
-        t.k, simt::BK,
-        [&](int r) -> const T* { return k0 + r < kmax ? k + (int64_t)(tok0 + k0 + r) * a.k_tok : nullptr; }, kvec, 1.f);
-    t.template fill<T>(
-        t.v, simt::BK,
-        [&](int r) -> const T* { return k0 + r < kmax ? v + (int64_t)(tok0 + k0 + r) * a.v_tok : nullptr; }, vvec, 1.f);
+    t.template fill_kv<T>(
+        [&](int r, const T*& ks, const T*& vs) {
+          if (k0 + r > last) return;
+          ks = k + (int64_t)(tok0 + k0 + r) * a.k_tok;
+          vs = v + (int64_t)(tok0 + k0 + r) * a.v_tok;
+        },
+        kvec, vvec);
     __syncthreads();
-    t.step(k0 + simt::BK > (int)(r0 / a.group) + 1,
-           [&](int r, int key) { return k0 + key <= (int)((r0 + r) / a.group); });
+    t.step(k0 + simt::BK > first + 1, [&](int i) -> uint64_t {
+      const int n = token[i] + 1 - k0;  // keys of the tile up to its own
+      return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+    });
   }
   T* out = reinterpret_cast<T*>(a.out);
 #pragma unroll
@@ -86,14 +93,14 @@ __global__ void __launch_bounds__(simt::kThreads) prompt_simt_kernel(const Args 
     const float L = t.row_sum(i);
     const int r = t.ty * 4 + i;
     if (r >= nr) continue;
-    const int64_t rr = r0 + r;
-    T* dst = out + (tok0 + rr / a.group) * a.o_tok + (hk * a.group + rr % a.group) * a.o_head;
+    T* dst = out + (int64_t)(tok0 + token[i]) * a.o_tok +
+             (int64_t)(hk * a.group + (r0 + r - (token[i] - it.z) * a.group)) * a.o_head;
     // a sum of zero (every score -inf) gives zero
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d = 4 * (t.tx + 16 * c);
-      float4 x = t.o[i][c];
+      float4 x = t.out(i, c);
       x.x *= inv;
       x.y *= inv;
       x.z *= inv;

@@ -8,12 +8,22 @@
 // V and the weights of a tile stand in shared memory as fp32 with rows padded
 // by 4 floats (16 lanes reading 16 rows' vectors touch every bank once per
 // quarter warp).  One pass over the keys with a running maximum and sum.
+//
+// Bound by the instructions of 8 warps that hide little of each other's latency:
+// products in pairs of columns (two fp32 results an instruction), a tile's loads
+// together, masks as bits per row.  8 prompts of 1000 tokens, 12 heads of 64: 480
+// us, 26 TFLOP/s (1080 us and 11 with 16 query rows per block instead of 64).
 #pragma once
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace pse {
 namespace simt {
+
+using t5::fma2;
+using t5::mul2;
+using t5::pack2;
+using t5::unpack2;
 
 constexpr int kThreads = 256;
 constexpr int BK = 64;
@@ -52,7 +62,7 @@ struct Tile {
   static constexpr int BQ = 16 * RPT;
   int hd, ld, tx, ty;
   float *q, *k, *v, *p;
-  float4 o[RPT][NC];
+  uint64_t o[RPT][NC][2];  // pairs of columns
   float m[RPT], l[RPT];
 
   __device__ void init(float* smem, int head_dim) {
@@ -71,58 +81,103 @@ struct Tile {
       m[i] = -INFINITY;
       l[i] = 0.f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < NC; ++c) o[i][c][0] = o[i][c][1] = 0ull;
     }
   }
-  // rows of `dst` from row_ptr(r) (nullptr: zeros); scale applied to the values
+  // Q from row(r) (nullptr: zeros), scaled.  Here and below a thread's loads are on
+  // their way together: one after the other their latency was most of a short
+  // item's time.
   template <typename T, typename F>
-  __device__ void fill(float* dst, int rows, F row_ptr, bool vec, float scale) {
+  __device__ void fill_q(F row, bool vec, float scale) {
     const int c4 = (hd + 3) / 4;
-    for (int e = threadIdx.x; e < rows * c4; e += kThreads) {
-      const int r = e / c4, d = (e - r * c4) * 4;
-      const T* src = row_ptr(r);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (src) x = load4<T>(src + d, hd - d, vec);
-      if (scale != 1.f) {
-        x.x *= scale;
-        x.y *= scale;
-        x.z *= scale;
-        x.w *= scale;
+#pragma unroll 1
+    for (int e0 = threadIdx.x; e0 < BQ * c4; e0 += RPT * kThreads) {
+      float4 x[RPT];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int e = min(e0 + i * kThreads, BQ * c4 - 1), r = e / c4, d = (e - r * c4) * 4;
+        const T* src = row(r);
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (src) x[i] = load4<T>(src + d, hd - d, vec);
       }
-      *reinterpret_cast<float4*>(dst + (size_t)r * ld + d) = x;
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int e = e0 + i * kThreads, r = e / c4, d = (e - r * c4) * 4;
+        if (e < BQ * c4)
+          *reinterpret_cast<float4*>(q + (size_t)r * ld + d) =
+              make_float4(x[i].x * scale, x[i].y * scale, x[i].z * scale, x[i].w * scale);
+      }
     }
   }
-  // One tile of BK keys (K, V and Q filled, a barrier passed).  visible(row,
-  // key) is asked only when `masked`; weights of hidden keys take no part, so
-  // what stands in a hidden key's V does not matter.
+  // BK rows of K and V; rows(r, ks, vs) sets their pointers (or leaves nullptr: zeros)
+  template <typename T, typename F>
+  __device__ void fill_kv(F rows, bool kvec, bool vvec) {
+    const int c4 = (hd + 3) / 4;
+#pragma unroll 1
+    for (int e0 = threadIdx.x; e0 < BK * c4; e0 += 4 * kThreads) {
+      float4 x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = min(e0 + i * kThreads, BK * c4 - 1), r = e / c4, d = (e - r * c4) * 4;
+        const T *ks = nullptr, *vs = nullptr;
+        rows(r, ks, vs);
+        x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ks) {
+          x[i] = load4<T>(ks + d, hd - d, kvec);
+          y[i] = load4<T>(vs + d, hd - d, vvec);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i * kThreads, r = e / c4, d = (e - r * c4) * 4;
+        if (e < BK * c4) {
+          *reinterpret_cast<float4*>(k + (size_t)r * ld + d) = x[i];
+          *reinterpret_cast<float4*>(v + (size_t)r * ld + d) = y[i];
+        }
+      }
+    }
+  }
+  // One tile of BK keys (K, V and Q filled, a barrier passed).  visible(i), asked
+  // only when `masked`, has a bit for each key that this thread's row i sees;
+  // weights of hidden keys take no part, so what stands in a hidden key's V does
+  // not matter.
   template <typename F>
   __device__ void step(bool masked, F visible) {
-    float s[RPT][4];
+    // (sums of the even and of the odd columns)
+    uint64_t s2[RPT][4];
 #pragma unroll
     for (int i = 0; i < RPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+      for (int j = 0; j < 4; ++j) s2[i][j] = 0ull;
     const int c4 = (hd + 3) / 4;
+#pragma unroll 4
     for (int c = 0; c < c4; ++c) {
-      float4 a[RPT], b[4];
+      ulonglong2 a[RPT], b[4];
 #pragma unroll
-      for (int i = 0; i < RPT; ++i) a[i] = *reinterpret_cast<const float4*>(q + (size_t)(ty * RPT + i) * ld + 4 * c);
+      for (int i = 0; i < RPT; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(q + (size_t)(ty * RPT + i) * ld + 4 * c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(k + (size_t)(tx + 16 * j) * ld + 4 * c);
+      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(k + (size_t)(tx + 16 * j) * ld + 4 * c);
 #pragma unroll
       for (int i = 0; i < RPT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+        for (int j = 0; j < 4; ++j) s2[i][j] = fma2(a[i].x, b[j].x, fma2(a[i].y, b[j].y, s2[i][j]));
     }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
+      float s[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float odd;
+        unpack2(s2[i][j], s[j], odd);
+        s[j] += odd;
+      }
       if (masked) {
+        const uint64_t vis = visible(i) >> tx;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (!visible(ty * RPT + i, tx + 16 * j)) s[i][j] = -INFINITY;
+          if (!(vis >> (16 * j) & 1ull)) s[j] = -INFINITY;
       }
-      float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+      float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float mn = fmaxf(m[i], mx), ms = mn == -INFINITY ? 0.f : mn;
@@ -131,19 +186,28 @@ struct Tile {
       l[i] *= corr;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        o[i][c].x *= corr;
-        o[i][c].y *= corr;
-        o[i][c].z *= corr;
-        o[i][c].w *= corr;
+        o[i][c][0] = mul2(o[i][c][0], pack2(corr, corr));
+        o[i][c][1] = mul2(o[i][c][1], pack2(corr, corr));
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float w = exp2f(s[i][j] - ms);
+        const float w = exp2f(s[j] - ms);
         l[i] += w;
         p[(ty * RPT + i) * (BK + 4) + tx + 16 * j] = w;
       }
     }
     __syncwarp();  // a row's weights are written and read by one half warp
+    if (masked)
+      values<true>();
+    else
+      values<false>();
+  }
+  // o += p v.  Columns past the head's are computed and not used (their reads end
+  // inside the tile's memory).  MASKED: a weight of zero takes no part, which
+  // matters where V is infinite or NaN.
+  template <bool MASKED>
+  __device__ __forceinline__ void values() {
+#pragma unroll 4
     for (int kk = 0; kk < BK; kk += 4) {
       float4 w[RPT];
 #pragma unroll
@@ -152,21 +216,31 @@ struct Tile {
       for (int x = 0; x < 4; ++x) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const int d = 4 * (tx + 16 * c);
-          if (d >= hd) continue;
-          const float4 b = *reinterpret_cast<const float4*>(v + (size_t)(kk + x) * ld + d);
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(v + (size_t)(kk + x) * ld + 4 * (tx + 16 * c));
+          bool skip = false;
+          if (MASKED) {
+            float f[4];
+            unpack2(b.x, f[0], f[1]);
+            unpack2(b.y, f[2], f[3]);
+            skip = !(fabsf(f[0]) + fabsf(f[1]) + fabsf(f[2]) + fabsf(f[3]) < INFINITY);
+          }
 #pragma unroll
           for (int i = 0; i < RPT; ++i) {
             const float y = x == 0 ? w[i].x : x == 1 ? w[i].y : x == 2 ? w[i].z : w[i].w;
-            if (masked && y == 0.f) continue;
-            o[i][c].x = fmaf(y, b.x, o[i][c].x);
-            o[i][c].y = fmaf(y, b.y, o[i][c].y);
-            o[i][c].z = fmaf(y, b.z, o[i][c].z);
-            o[i][c].w = fmaf(y, b.w, o[i][c].w);
+            if (skip && y == 0.f) continue;
+            o[i][c][0] = fma2(pack2(y, y), b.x, o[i][c][0]);
+            o[i][c][1] = fma2(pack2(y, y), b.y, o[i][c][1]);
           }
         }
       }
     }
+  }
+  // columns 4 (tx + 16 c) .. + 3 of the thread's row i
+  __device__ float4 out(int i, int c) const {
+    float4 x;
+    unpack2(o[i][c][0], x.x, x.y);
+    unpack2(o[i][c][1], x.z, x.w);
+    return x;
   }
   // the row's sum over its 16 lanes
   __device__ float row_sum(int i) const {

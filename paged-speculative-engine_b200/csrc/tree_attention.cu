@@ -169,7 +169,7 @@ template <typename T, int RPT, int NC>
 __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a) {
   extern __shared__ float smem[];
   __shared__ int tmp[36];
-  constexpr int BQ = 16 * RPT, TILE = simt::BK;
+  constexpr int TILE = simt::BK;
   Span span;
   const Split split = my_span<TILE>(a.rows, a.block_nodes, tmp, span);
   Cut cut{-1, 0, 0, 0};
@@ -181,20 +181,21 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
   };
   const bool qvec = aligned(a.q, a.q_tok, a.q_head);
   const bool kvec = aligned(a.k_pool, hd, hd), vvec = aligned(a.v_pool, hd, hd);
+  int rt[RPT];  // the node of each of this thread's rows
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) rt[i] = (t.ty * RPT + i) / group;
   Walk<TILE> walk;
   walk.start(a.rows, span, a.block_nodes);
   Segment g;
   while (walk.next(g)) {
-    // rows of the block: (node, group head), node-major; a group above BQ heads
-    // takes its rows BQ at a time
+    // rows of the block: (node, group head), node-major
     const int node0 = g.block * a.block_nodes;
     const int nr = min(a.block_nodes, g.r.nodes - node0) * group;
     const int32_t* table = a.block_table + (int64_t)max(g.r.slot, 0) * a.max_blocks;
     const int held = g.r.slot >= 0 ? min(a.nblocks[g.r.slot], a.max_blocks) : 0;
     t.reset();
     __syncthreads();
-    t.template fill<T>(
-        t.q, BQ,
+    t.template fill_q<T>(
         [&](int r) -> const T* {
           if (r >= nr) return nullptr;
           return reinterpret_cast<const T*>(a.q) + (int64_t)(g.r.n0 + node0 + r / group) * a.q_tok +
@@ -205,24 +206,26 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
     for (int tile = g.t0; tile < g.t1; ++tile) {
       const int k0 = tile * TILE;
       __syncthreads();
-      auto at = [&](const char* pool, int r) -> const T* {
-        const int key = k0 + r;
-        if (key >= keys) return nullptr;
-        const int bi = key / a.block_size;
-        if (bi >= held) return nullptr;
-        const int blk = table[bi];
-        if (blk < 0 || blk >= a.num_blocks) return nullptr;
-        return reinterpret_cast<const T*>(pool) +
-               (((int64_t)blk * a.rows.kv_heads + g.hk) * a.block_size + key % a.block_size) * hd;
-      };
-      t.template fill<T>(t.k, TILE, [&](int r) { return at(a.k_pool, r); }, kvec, 1.f);
-      t.template fill<T>(t.v, TILE, [&](int r) { return at(a.v_pool, r); }, vvec, 1.f);
+      t.template fill_kv<T>(
+          [&](int r, const T*& ks, const T*& vs) {
+            const int key = k0 + r;
+            if (key >= keys) return;
+            const int bi = key / a.block_size;
+            if (bi >= held) return;
+            const int blk = __ldg(table + bi);
+            if (blk < 0 || blk >= a.num_blocks) return;
+            const int64_t at = (((int64_t)blk * a.rows.kv_heads + g.hk) * a.block_size + (key - bi * a.block_size)) * hd;
+            ks = reinterpret_cast<const T*>(a.k_pool) + at;
+            vs = reinterpret_cast<const T*>(a.v_pool) + at;
+          },
+          kvec, vvec);
       __syncthreads();
-      t.step(k0 + TILE > g.r.ctx || g.r.slot < 0, [&](int r, int key) {
-        if (r >= nr || k0 + key >= keys) return false;
-        const uint32_t* m = reinterpret_cast<const uint32_t*>(a.masks + (int64_t)(g.r.n0 + node0 + r / group) * a.words);
-        const auto word = [&](int i) { return __ldg(m + i); };
-        return (visible32(word, a.words, g.r.slot, g.r.ctx, g.r.nodes, k0 + (key & ~31)) >> (key & 31) & 1u) != 0u;
+      t.step(k0 + TILE > g.r.ctx || g.r.slot < 0, [&](int i) -> uint64_t {
+        if (t.ty * RPT + i >= nr) return 0ull;
+        const uint32_t* m = reinterpret_cast<const uint32_t*>(a.masks + (int64_t)(g.r.n0 + node0 + rt[i]) * a.words);
+        const auto word = [&](int w) { return __ldg(m + w); };
+        const uint32_t lo = visible32(word, a.words, g.r.slot, g.r.ctx, g.r.nodes, k0);
+        return lo | (uint64_t)visible32(word, a.words, g.r.slot, g.r.ctx, g.r.nodes, k0 + 32) << 32;
       });
     }
     T* out = reinterpret_cast<T*>(a.out);
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
       for (int c = 0; c < NC; ++c) {
         const int d = 4 * (t.tx + 16 * c);
         if (d >= hd) continue;
-        float4 x = t.o[i][c];
+        float4 x = t.out(i, c);
         if (whole) {
           x.x *= inv;
           x.y *= inv;
