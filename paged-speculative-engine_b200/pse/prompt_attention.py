@@ -10,7 +10,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from .rotary import head_view
+from .rotary import head_view, new_result
 
 
 class PackedPrompts:
@@ -82,8 +82,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompts:
     vv = head_view("v", v, T, prompts.kv_heads, hd, dtype, dev)
     code = N.dtype_code(dtype)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ov = head_view("out", out, T, prompts.q_heads, hd, dtype, dev)
+        out, ov = new_result(q, qv, hd)
+    else:
+        ov = head_view("out", out, T, prompts.q_heads, hd, dtype, dev)
     rc = prompts.fn(qv, kv, vv, ov, T, hd, code, 1.0 / math.sqrt(hd) if scale is None else float(scale),
                     prompts._plan_ptr, prompts.n_cta, prompts.n_items, prompts._status_ptr, N.stream_ptr())
     if rc:

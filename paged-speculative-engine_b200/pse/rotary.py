@@ -139,6 +139,13 @@ def index_ptr(name: str, t: torch.Tensor, n: int, device: int) -> int:
     return t.data_ptr()
 
 
+def new_result(src: torch.Tensor, view: N.HeadView, head_dim: int):
+    """A contiguous result tensor of the shape of ``src`` ([tokens, heads,
+    head_dim], checked as ``view``) and the library's view of it."""
+    out, heads = torch.empty_like(src, memory_format=torch.contiguous_format), view.heads
+    return out, N.HeadView(out.data_ptr(), heads * head_dim, head_dim, heads)
+
+
 def _out_view(name: str, out: torch.Tensor, src: torch.Tensor, view: N.HeadView, head_dim: int, dtype, device: int):
     v = head_view(name, out, src.shape[0], view.heads, head_dim, dtype, device)
     if v.data == view.data and (v.tok_stride != view.tok_stride or v.head_stride != view.head_stride) and src.numel():
@@ -157,14 +164,16 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     code, T = N.dtype_code(dtype), q.shape[0]
     pos = index_ptr("positions", positions, T, dev)
     if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
+        q_out, qo = new_result(q, qv, hd)
+    else:
+        qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
     kv = ko = _NO_HEADS
     if k is not None:
         kv = head_view("k", k, T, None, hd, dtype, dev)
         if k_out is None:
-            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-        ko = _out_view("k_out", k_out, k, kv, hd, dtype, dev)
+            k_out, ko = new_result(k, kv, hd)
+        else:
+            ko = _out_view("k_out", k_out, k, kv, hd, dtype, dev)
     rc = plan.fn(plan.spec, qv, qo, kv, ko, pos, T, code, N.stream_ptr())
     if rc:
         raise N.failed("pse_rotary", rc)
@@ -194,8 +203,9 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     slot = index_ptr("slots", slots, T, dev)
     at = index_ptr("cache_positions", cache_positions, T, dev)
     if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
+        q_out, qo = new_result(q, qv, hd)
+    else:
+        qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
     ko = _NO_HEADS if k_out is None else _out_view("k_out", k_out, k, kv, hd, dtype, dev)
     rc = plan.append_fn(cache.state, cache.layer(layer), plan.spec, qv, qo, kv, ko, vv, pos, slot, at, T,
                         N.stream_ptr())

@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _native as N
-from .rotary import head_view, index_ptr
+from .rotary import head_view, index_ptr, new_result
 
 MAX_NODES = 4096  # nodes of one request's tree
 
@@ -39,8 +39,9 @@ class TokenTrees:
             raise ValueError(f"{self.words} mask words for a tree of {self.max_nodes} nodes")
         self.masks, self.depths, self.device, self.index = masks, depths, masks.device, masks.get_device()
         self.offsets = _offsets(self.counts, self.device) if offsets is None else offsets
+        self._offsets_ptr = index_ptr("offsets", self.offsets, len(self.counts) + 1, self.index)
         self.fn = N.fn("pse_token_tree_attention")
-        self._masks_ptr, self._offsets_ptr = masks.data_ptr(), self.offsets.data_ptr()
+        self._masks_ptr = masks.data_ptr()
 
     @classmethod
     def from_parents(cls, parents: torch.Tensor, counts) -> "TokenTrees":
@@ -109,10 +110,13 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
         raise ValueError(f"{heads} query heads over {cache.n_heads} K/V heads of {hd}")
     slot, ctx = index_ptr("slots", slots, rows, dev), index_ptr("context", context, rows, dev)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ov = head_view("out", out, trees.nodes, heads, hd, dtype, dev)
+        out, ov = new_result(q, qv, hd)
+    else:
+        ov = head_view("out", out, trees.nodes, heads, hd, dtype, dev)
     if workspace is None:
         workspace = token_tree_workspace(hd, q.device)
+    elif workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on GPU {dev}")
     rc = trees.fn(cache.state, cache.layer(layer), qv, ov, slot, ctx, trees._offsets_ptr, rows, trees.nodes,
                   trees.max_nodes, trees._masks_ptr, trees.words, 1.0 / math.sqrt(hd) if scale is None else float(scale),
                   workspace.data_ptr(), workspace.numel(), N.stream_ptr())

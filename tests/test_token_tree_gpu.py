@@ -291,3 +291,18 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         pse.token_tree_attention(c.q, c.cache, 0, slots, c.context, c.trees,
                                  workspace=torch.zeros(64, dtype=torch.uint8, device="cuda"))
+
+
+def test_refusals_of_kept_buffers():
+    """A workspace or offsets that the kernel cannot use are refused before the launch."""
+    import pse
+    c = Case([5, 9], [3, 2], 4, 2, 64, 16, torch.bfloat16, 1)
+    size = pse.token_tree.token_tree_workspace(64, "cuda").numel()
+    for bad in (torch.zeros(size, dtype=torch.uint8), torch.zeros(size, dtype=torch.int32, device="cuda"),
+                torch.zeros(2 * size, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError):
+            c.run(workspace=bad)
+    for bad in (torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32),
+                torch.zeros(3, dtype=torch.int64, device="cuda")):
+        with pytest.raises(ValueError):
+            pse.TokenTrees(c.trees.masks, c.nodes, offsets=bad)
