@@ -34,22 +34,27 @@ struct Args {
   int block_nodes;
   float scale_log2;
   Cut* cuts;     // [workers]
-  float* parts;  // [workers][2][part_rows][hd + 2]
+  float* parts;  // [workers][2][part_rows * part_width(hd)]
   int part_rows;
   int32_t* status;
   bool out_vec;  // output rows are 16-byte aligned
 };
 
-// Partial results of cut items: per worker two blocks of `part_rows` rows of hd
-// columns, then a (maximum, sum) per row.  A worker's first segment, if it begins
-// inside an item, uses the first block; a segment that begins an item and does
-// not end it, necessarily the worker's last, uses the second.
+// Partial results of cut items: per worker two blocks of `part_rows` rows, first
+// the output four columns at a time (a float4 of every row, then the next four
+// columns: threads with a row each write and read them side by side), then a
+// (maximum, sum) per row.  A worker's first segment, if it begins inside an item,
+// uses the first block; a segment that begins an item and does not end it,
+// necessarily the worker's last, uses the second.
+__host__ __device__ constexpr int part_width(int hd) { return (hd + 3) / 4 * 4 + 2; }  // floats per row
 __device__ __forceinline__ float* part(const Args& a, int cta, bool starts_item) {
-  return a.parts + ((int64_t)cta * 2 + (starts_item ? 1 : 0)) * a.part_rows * (a.hd + 2);
+  return a.parts + ((int64_t)cta * 2 + (starts_item ? 1 : 0)) * a.part_rows * part_width(a.hd);
 }
-__device__ __forceinline__ float* part_row(const Args& a, float* block, int r) { return block + (int64_t)r * a.hd; }
-__device__ __forceinline__ float* part_stats(const Args& a, float* block, int r) {
-  return block + (int64_t)a.part_rows * a.hd + 2 * r;
+__device__ __forceinline__ float4* part_cols(const Args& a, float* block, int r, int col) {  // col: a multiple of 4
+  return reinterpret_cast<float4*>(block) + col / 4 * a.part_rows + r;
+}
+__device__ __forceinline__ float2* part_stats(const Args& a, float* block, int r) {
+  return reinterpret_cast<float2*>(block + a.part_rows * (part_width(a.hd) - 2)) + r;
 }
 
 // What the join needs of the item that worker c begins and does not end.
@@ -60,95 +65,90 @@ struct Cut {
   int hk;
 };
 
-// A warp per row of the cut items, lanes over the columns: the parts are summed
-// in the order of their workers.  Every block reads all cuts and numbers their
-// rows, so the rows are spread over the whole GPU whatever was cut where.  (A
-// block per cut and row slice instead, most of them idle, took 28 us where this
-// takes 9, two trees of 64 nodes with 8192 tokens each.)
+// A warp per 32 rows and 8 columns of a cut item, a row per lane: the parts are
+// summed in the order of their workers.  Every block reads all cuts and numbers
+// their tasks, so these are spread over the whole GPU whatever was cut where.
+// (A warp per row with its lanes over the columns, the parts row by row, took 10 us
+// more where 64 rows-per-head trees of 2048 tokens leave 31 thousand cut rows: the
+// parts' writer, a thread per row, then writes 16 bytes to each of 32 lines.)
 constexpr int kJoinThreads = 512;
 
-template <typename T, int PER>
+template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, int workers, int tile_rows, int tile_pitch) {
   __shared__ int scan_tmp[33];
-  __shared__ int first_row[kJoinThreads];  // rows of the cuts before
+  __shared__ int first_chunk[kJoinThreads];  // chunks of 32 rows of the cuts before
   __shared__ int4 cuts[kJoinThreads];
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, group = a.rows.group, hd = a.hd;
   int4 mine = make_int4(-1, 0, 0, 0);
   if (tid < workers) mine = __ldcg(reinterpret_cast<const int4*>(a.cuts + tid));
   int total;
-  const int before = block_exclusive_scan(mine.x >= 0 ? mine.z * group : 0, scan_tmp, &total);
-  first_row[tid] = before;
+  const int before = block_exclusive_scan(mine.x >= 0 ? ceil_div(mine.z * group, 32) : 0, scan_tmp, &total);
+  first_chunk[tid] = before;
   cuts[tid] = mine;
   __syncthreads();
-  const int warps = gridDim.x * (kJoinThreads / 32);
+  const int warps = gridDim.x * (kJoinThreads / 32), col_groups = ceil_div(hd, 8);
 #pragma unroll 1
-  for (int task = blockIdx.x * (kJoinThreads / 32) + (tid >> 5); task < total; task += warps) {
-    // the last cut whose rows begin at or before the task (cuts without rows share
-    // their successor's beginning)
+  for (int task = blockIdx.x * (kJoinThreads / 32) + (tid >> 5); task < total * col_groups; task += warps) {
+    const int chunk = task / col_groups, col = 8 * (task - chunk * col_groups);
+    // the last cut whose chunks begin at or before this one (cuts without rows
+    // share their successor's beginning)
     int c1 = 0;
 #pragma unroll
     for (int step = kJoinThreads / 2; step > 0; step >>= 1)
-      if (first_row[c1 + step] <= task) c1 += step;
+      if (first_chunk[c1 + step] <= chunk) c1 += step;
     const int4 cut = cuts[c1];
-    const int c2 = cut.x, row = task - first_row[c1];
+    const int n = cut.x - c1 + 1;
+    const int row = 32 * (chunk - first_chunk[c1]) + lane;
+    if (row >= cut.z * group) continue;
     const int r = row / tile_rows * tile_pitch + row % tile_rows;
+    const bool second = col + 4 < hd;
     // worker c1 holds the item's beginning in its second block, the others theirs
     // in their first
-    const int64_t pitch = 2ll * a.part_rows * (hd + 2);
-    const float* base = a.parts + c1 * pitch + (int64_t)a.part_rows * (hd + 2);
-    auto block = [&](int i) -> const float* {  // of worker c1 + i
-      return i == 0 ? base : base + i * pitch - (int64_t)a.part_rows * (hd + 2);
-    };
-    const int64_t stats = (int64_t)a.part_rows * hd + 2 * r;
-    const int n = c2 - c1 + 1;
-    // four parts' values on their way before the statistics that weigh them
-    float v[4][PER];
+    auto block = [&](int i) { return part(a, c1 + i, i == 0); };
+    // four parts on their way at a time
+    float2 ml[4];
+    float4 x[4], y[4];
     auto load = [&](int i0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float* p = block(min(i0 + i, n - 1)) + (int64_t)r * hd;
-#pragma unroll
-        for (int y = 0; y < PER; ++y) v[i][y] = lane + 32 * y < hd ? __ldcg(p + lane + 32 * y) : 0.f;
+        float* p = block(min(i0 + i, n - 1));
+        ml[i] = __ldcg(part_stats(a, p, r));
+        x[i] = __ldcg(part_cols(a, p, r, col));
+        y[i] = second ? __ldcg(part_cols(a, p, r, col + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     };
     load(0);
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < n) ml = __ldcg(reinterpret_cast<const float2*>(block(lane) + stats));
-    float M = ml.x;
+    float M = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));  // (past n: the last part's once more)
 #pragma unroll 1
-    for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, __ldcg(block(i) + stats));
-    M = warp_max(M);
+    for (int i = 4; i < n; ++i) M = fmaxf(M, __ldcg(part_stats(a, block(i), r)).x);
     const float ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    float L = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += 4) {
-      if (i0 > 0) {
-        load(i0);
-        if ((i0 & 31) == 0) {
-          ml = make_float2(-INFINITY, 0.f);
-          if (i0 + lane < n) ml = __ldcg(reinterpret_cast<const float2*>(block(i0 + lane) + stats));
-        }
-      }
-      const float f = exp2f(ml.x - ms), l = ml.y * f;  // a sum is finite or the NaN of a score
+      if (i0 > 0) load(i0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i0 + i >= n) break;
-        const float fi = __shfl_sync(0xffffffffu, f, (i0 + i) & 31);
-        L += __shfl_sync(0xffffffffu, l, (i0 + i) & 31);
+        const float f = exp2f(ml[i].x - ms);
+        L += ml[i].y * f;  // a sum is finite or the NaN of a score
+        const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
 #pragma unroll
-        for (int y = 0; y < PER; ++y) acc[y] += fi == 0.f ? 0.f : v[i][y] * fi;
+        for (int d = 0; d < 8; ++d) acc[d] += f == 0.f ? 0.f : v[d] * f;
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     T* dst = reinterpret_cast<T*>(a.out) + (int64_t)(cut.y + row / group) * a.o_tok +
-             (int64_t)(cut.w * group + row % group) * a.o_head;
+             (int64_t)(cut.w * group + row % group) * a.o_head + col;
 #pragma unroll
-    for (int y = 0; y < PER; ++y) {
-      const int d = lane + 32 * y;
-      if (d < hd) dst[d] = from_f32<T>(acc[y] * inv);
+    for (int d = 0; d < 8; ++d) acc[d] *= inv;
+    if (sizeof(T) == 2 && a.out_vec && col + 8 <= hd) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(t5::pack_bf16(acc[0], acc[1]), t5::pack_bf16(acc[2], acc[3]),
+                                                  t5::pack_bf16(acc[4], acc[5]), t5::pack_bf16(acc[6], acc[7]));
+    } else {
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+        if (col + d < hd) dst[d] = from_f32<T>(acc[d]);
     }
   }
 }
@@ -156,11 +156,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, int wo
 template <typename T>
 int launch_join(const Args& a, int workers, int tile_rows, int tile_pitch, cudaStream_t s) {
   static_assert(kMaxWorkers <= kJoinThreads, "a thread per cut");
-  const dim3 grid(3 * kNumSMs), block(kJoinThreads);
   const cudaError_t e =
-      a.hd <= 64    ? launch_pdl(join_kernel<T, 2>, grid, block, 0, s, a, workers, tile_rows, tile_pitch)
-      : a.hd <= 128 ? launch_pdl(join_kernel<T, 4>, grid, block, 0, s, a, workers, tile_rows, tile_pitch)
-                    : launch_pdl(join_kernel<T, 8>, grid, block, 0, s, a, workers, tile_rows, tile_pitch);
+      launch_pdl(join_kernel<T>, dim3(2 * kNumSMs), dim3(kJoinThreads), 0, s, a, workers, tile_rows, tile_pitch);
   return e == cudaSuccess ? PSE_OK : (int)e;
 }
 
@@ -254,13 +251,10 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
           x.w *= inv;
           simt::store4(out_row(r) + d, hd - d, x);
         } else {
-          simt::store4(part_row(a, mine, r) + d, hd - d, x);
+          *part_cols(a, mine, r, d) = x;
         }
       }
-      if (!whole && t.tx == 0) {
-        part_stats(a, mine, r)[0] = t.m[i];
-        part_stats(a, mine, r)[1] = L;
-      }
+      if (!whole && t.tx == 0) *part_stats(a, mine, r) = make_float2(t.m[i], L);
     }
   }
   if (threadIdx.x == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(cut.last, cut.node0, cut.nodes, cut.hk);
@@ -511,12 +505,12 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
         if (valid && whole) {
           tile::store_row32(dst + col, o, inv, a.out_vec);
         } else if (valid) {
-          float4* p = reinterpret_cast<float4*>(part_row(a, mine, prow) + col);
 #pragma unroll
-          for (int y = 0; y < 8; ++y) __stcg(p + y, make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]));
+          for (int y = 0; y < 8; ++y)
+            __stcg(part_cols(a, mine, prow, col + 4 * y), make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]));
         }
       }
-      if (!whole && valid) __stcg(reinterpret_cast<float2*>(part_stats(a, mine, prow)), make_float2(row.m, row.l));
+      if (!whole && valid) __stcg(part_stats(a, mine, prow), make_float2(row.m, row.l));
       // the output and the segment's description have been read
       fence_before();
       __syncwarp();
@@ -833,7 +827,7 @@ extern "C" size_t pse_token_tree_workspace(int32_t head_dim) {
   if (head_dim <= 0) return 0;
   // two partial results per CTA: of 64 rows on the CUDA cores, of 256 on the tensor cores
   const size_t simt = (size_t)tree::kMaxWorkers * 64, tc = (size_t)kNumSMs * 256;
-  return tree::kCutBytes + (head_dim <= 128 && tc > simt ? tc : simt) * 2 * (head_dim + 2) * 4;
+  return tree::kCutBytes + (head_dim <= 128 && tc > simt ? tc : simt) * 2 * tree::part_width(head_dim) * 4;
 }
 
 extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,
