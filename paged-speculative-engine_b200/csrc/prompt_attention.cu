@@ -218,6 +218,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
   if (tid == 0) {
+    prefetch_map(&tmq);
+    prefetch_map(&tmk);
+    prefetch_map(&tmv);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&slot_full[i], 1);
       mbar_init(&slot_empty[i], 1);
@@ -246,6 +249,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  pdl_trigger();
   const int tpt = tile_tokens(a.group);
   const int e0 = __ldg(a.plan + blockIdx.x), e1 = min(__ldg(a.plan + blockIdx.x + 1), a.n_items);
 

@@ -99,6 +99,9 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) { mbar_drain(su32(bar), parity); }
 
 // ---------------------------------------------------------------- TMA
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"

@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, int wo
   __shared__ int first_chunk[kJoinThreads];  // chunks of 32 rows of the cuts before
   __shared__ int4 cuts[kJoinThreads];
   pdl_wait();
+  pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, group = a.rows.group, hd = a.hd;
   int4 mine = make_int4(-1, 0, 0, 0);
   if (tid < workers) mine = __ldcg(reinterpret_cast<const int4*>(a.cuts + tid));
@@ -112,14 +113,17 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, int wo
     auto load = [&](int i0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float* p = block(min(i0 + i, n - 1));
+        ml[i] = make_float2(-INFINITY, 0.f);
+        x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + i >= n) continue;
+        float* p = block(i0 + i);
         ml[i] = __ldcg(part_stats(a, p, r));
         x[i] = __ldcg(part_cols(a, p, r, col));
-        y[i] = second ? __ldcg(part_cols(a, p, r, col + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (second) y[i] = __ldcg(part_cols(a, p, r, col + 4));
       }
     };
     load(0);
-    float M = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));  // (past n: the last part's once more)
+    float M = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
 #pragma unroll 1
     for (int i = 4; i < n; ++i) M = fmaxf(M, __ldcg(part_stats(a, block(i), r)).x);
     const float ms = M == -INFINITY ? 0.f : M;
@@ -165,8 +169,9 @@ int launch_join(const Args& a, int workers, int tile_rows, int tile_pitch, cudaS
 template <typename T, int RPT, int NC>
 __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a) {
   extern __shared__ float smem[];
-  __shared__ int tmp[36];
+  __shared__ int tmp[40];
   constexpr int TILE = simt::BK;
+  pdl_trigger();
   Span span;
   const Split split = my_span<TILE>(a.rows, a.block_nodes, tmp, span);
   Cut cut{-1, 0, 0, 0};
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
   constexpr int kTileBytes = 128 * HD * 2, kHalves = HD / 64;
   constexpr uint32_t kColO = 128 * NQ, kTmem = 256 * NQ;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int span_tmp[36];
+  __shared__ int span_tmp[40];
   __shared__ Seg segs[kSegs];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;                      // [NQ][128 x HD]
@@ -370,6 +375,9 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
   if (tid == 0) {
+    prefetch_map(&tmq);
+    prefetch_map(&tmk);
+    prefetch_map(&tmv);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&slot_full[i], 1);
       mbar_init(&slot_empty[i], 1);
@@ -398,6 +406,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
   fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  pdl_trigger();  // the join's blocks stand ready wherever this kernel's have ended
   Span span;
   const Split split = my_span<128>(a.rows, a.block_nodes, span_tmp, span);
   const int group = a.rows.group, tpt = 128 / group;
@@ -612,13 +621,14 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
       while (run && walk.next(g)) {
         const int g0 = guard_from(g), keys = g.r.ctx + g.r.nodes;
         const int32_t* table = a.block_table + (int64_t)max(g.r.slot, 0) * a.max_blocks;
-        const int held = g.r.slot >= 0 ? min(a.nblocks[g.r.slot], a.max_blocks) : 0;
-        // the pool rows of 32 pages (32 / ppt tiles), a page per lane, and of the next 32
+        const int held = g.r.slot >= 0 ? a.nblocks[g.r.slot] : 0;
+        // the pool rows of 32 pages (32 / ppt tiles), a page per lane, and of the next
+        // 32; the first ones' loads and that of `held` do not wait for each other
         auto page = [&](int j) -> int {
           const int pi = g.t0 * ppt + j;
-          if (pi >= g.t1 * ppt || pi >= held || pi * bs >= keys) return oob;
+          if (g.r.slot < 0 || pi >= g.t1 * ppt || pi >= a.max_blocks || pi * bs >= keys) return oob;
           const int b = __ldg(table + pi);
-          return b >= 0 && b < a.num_blocks ? (b * a.rows.kv_heads + g.hk) * bs : oob;
+          return pi < held && b >= 0 && b < a.num_blocks ? (b * a.rows.kv_heads + g.hk) * bs : oob;
         };
         int cur = page(lane), nxt = page(32 + lane);
 #pragma unroll 1

@@ -66,6 +66,7 @@ struct Split {
 struct Span {
   int begin, end;    // a worker's tiles
   int row, off;      // row of the first tile, and its offset within the row
+  Row r;             // that row
 };
 
 template <int TILE>
@@ -74,16 +75,21 @@ __device__ __forceinline__ int row_weight(const Rows& a, const Row& r, int block
 }
 
 // The span of this CTA, worker blockIdx.x of gridDim.x.  All threads of the CTA;
-// `tmp` holds 36 ints of shared memory.
+// `tmp` holds 40 ints of shared memory.
 template <int TILE>
 __device__ Split my_span(const Rows& a, int block_nodes, int* tmp, Span& x) {
   const int per = (a.rows + blockDim.x - 1) / blockDim.x;
   const int lo = min(a.rows, (int)threadIdx.x * per), hi = min(a.rows, lo + per);
   int mine = 0, first = 0;
+  Row r{-1, 0, 0, 0};  // row lo
 #pragma unroll 1
   for (int i = lo; i < hi; ++i) {
-    const int w = row_weight<TILE>(a, read_row(a, i), block_nodes);
-    if (i == lo) first = w;
+    const Row ri = read_row(a, i);
+    const int w = row_weight<TILE>(a, ri, block_nodes);
+    if (i == lo) {
+      first = w;
+      r = ri;
+    }
     mine += w;
   }
   // exclusive prefix over the threads
@@ -104,6 +110,7 @@ __device__ Split my_span(const Rows& a, int block_nodes, int* tmp, Span& x) {
   s.extra = total - s.per * s.workers;
   const int c = blockIdx.x;
   x.begin = x.end = x.row = x.off = 0;
+  x.r = Row{-1, 0, 0, 0};
   if (c < s.workers) {
     x.begin = s.per * c + min(c, s.extra);
     x.end = x.begin + s.per + (c < s.extra ? 1 : 0);
@@ -112,16 +119,22 @@ __device__ Split my_span(const Rows& a, int block_nodes, int* tmp, Span& x) {
 #pragma unroll 1
       while (at >= w) {
         at -= w;
-        w = row_weight<TILE>(a, read_row(a, ++i), block_nodes);
+        r = read_row(a, ++i);
+        w = row_weight<TILE>(a, r, block_nodes);
       }
       tmp[32] = i;
       tmp[33] = at;
+      tmp[34] = r.slot;
+      tmp[35] = r.ctx;
+      tmp[36] = r.n0;
+      tmp[37] = r.nodes;
     }
   }
   __syncthreads();
   if (c < s.workers) {
     x.row = tmp[32];
     x.off = tmp[33];
+    x.r = Row{tmp[34], tmp[35], tmp[36], tmp[37]};
   }
   return s;
 }
@@ -159,10 +172,10 @@ struct Walk {
     end = span.end;
     row = span.row;
     off = span.off;
-    if (at < end) load();
+    r = span.r;
+    weigh();
   }
-  __device__ __forceinline__ void load() {
-    r = read_row(*rows, row);
+  __device__ __forceinline__ void weigh() {
     nt = key_tiles<TILE>(r);
     nb = q_blocks(*rows, r, block_nodes);
     w = nt * nb * rows->kv_heads;
@@ -173,7 +186,8 @@ struct Walk {
     while (off >= w) {
       off -= w;
       if (++row >= rows->rows) return false;
-      load();
+      r = read_row(*rows, row);
+      weigh();
     }
     const int item = off / nt;
     g.r = r;
