@@ -109,8 +109,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t lane_base, uint32_t s_col,
 
 // The same in rolled loops of 32 columns, the scores read twice: a quarter of the
 // code and of the registers.  For kernels whose warps come back to a tile after
-// much other code: there the instructions' own way through the caches counts
-// (the token tree kernel lost a third of its time to it).
+// much other code: there the instructions' own way through the caches counts (64
+// trees of 5 to 26 nodes: 54 us, and 77 with the unrolled form above).
 template <int HD>
 __device__ __forceinline__ void softmax_tile_small(uint32_t lane_base, uint32_t s_col, uint32_t o_col, float sl2,
                                                    bool first, bool masked, uint32_t vis0, uint32_t vis1, uint32_t vis2,

@@ -8,10 +8,11 @@
 // Bound by HBM: every element is read once and written once.  A thread owns
 // one unit of a head, two 16-byte vectors (V pairs), for kHeads heads of one
 // token, and issues all its loads first; while they are in flight the block
-// computes its tokens' sines and cosines, each once, into shared memory.  The angle is kept in turns
-// and reduced in fp64 (one multiply, one rounding, one subtraction), so the
-// fp32 sine and cosine are those of the exact angle at any int32 position; no
-// table is read.
+// computes its tokens' sines and cosines, each once, into shared memory (105 us
+// where each thread computed its own, 62 so, at the size below: 5.4 TB/s).  The
+// angle is kept in turns and reduced in fp64 (one multiply, one rounding, one
+// subtraction), so the fp32 sine and cosine are those of the exact angle at any
+// int32 position; no table is read.
 #include "common.cuh"
 
 namespace pse {

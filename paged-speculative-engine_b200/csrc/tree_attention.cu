@@ -5,7 +5,15 @@
 // bits, one word per 64 nodes, and rows may hold different numbers of nodes.
 //
 // The context's K/V is read from HBM once per request, which bounds the call
-// until a K/V head has about 256 query rows (nodes x group).
+// until a K/V head has about 256 query rows (nodes x group).  Measured: 16
+// requests of 16384 tokens, 8 K/V heads of 128: 8 nodes (32 rows) 178 us (6.0
+// TB/s, 92% of a copy's rate), 32 nodes (128 rows) 197 us, 64 nodes (256 rows) 277
+// us (990 TFLOP/s, the products and the softmax in turn).  At head_dim 64 a row of
+// scores costs twice as many exponentials for its bytes, and the softmax warps
+// bound the call: 64 requests of 2048 tokens with 26 nodes 85 us (3.4 TB/s), with 6
+// nodes 66 us (4.1 TB/s).  A small tree (8 nodes, 300 tokens) takes 11 us, of which
+// 5 pass before the first scores stand (launch, the split of the work, the first
+// loads) and 3 in the join.
 #include "attention_tile.cuh"
 #include "simt_attention.cuh"
 #include "tmap_cache.h"
@@ -265,7 +273,10 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
   if (threadIdx.x == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(cut.last, cut.node0, cut.nodes, cut.hk);
 }
 
-int simt_rows(int rows) { return rows <= 16 ? 1 : 4; }
+// Rows per thread: blocks of 16 query rows up to 32, of 64 above (26 rows: 52
+// against 63 us, 104 rows: 684 against 413 us; 8 requests of 500 tokens and 12 K/V
+// heads, 16 of 2000 and 8).
+int simt_rows(int rows, int group) { return rows <= 32 && group <= 16 ? 1 : 4; }
 
 template <typename T, int RPT, int NC>
 int launch_simt(const Args& a, int grid, cudaStream_t s) {
@@ -288,7 +299,7 @@ int simt_nc(const Args& a, int grid, cudaStream_t s) {
 
 template <typename T>
 int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
-  const int rpt = simt_rows(max_nodes * a.rows.group);
+  const int rpt = simt_rows(max_nodes * a.rows.group, a.rows.group);
   a.block_nodes = 16 * rpt / a.rows.group;
   a.part_rows = 16 * rpt;
   if (!countable(a.rows, simt::BK, a.block_nodes)) return PSE_EINVAL;
@@ -316,6 +327,9 @@ int simt_attention(Args& a, int max_nodes, cudaStream_t s) {
 //               infinities and NaN before the product, as in prompt_attention.cu
 //   h + 3       Q tiles, so that the ring runs on into the next segment, and what
 //               the softmax and product warps have to know of it (Seg)
+// NQ = 1 keeps its softmax in rolled loops (softmax_tile_small).  Slower, 64 trees
+// of 26 nodes over 2048 tokens (85 us): scores of 64 keys in two buffers, two tiles
+// ahead of the values (89); halves of 64 scores in registers, 8 warps (91).
 using namespace t5;
 
 constexpr int kHalfBytes = 128 * 128;
@@ -764,7 +778,7 @@ bool tc_eligible(const Args& a, int q_heads) {
 }
 
 template <int HD, int NQ>
-int launch_tc(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
+int launch_tc(Args& a, int q_heads, cudaStream_t s) {
   auto kern = tree_tc_kernel<HD, NQ>;
   constexpr size_t smem = tc_smem_bytes<HD, NQ>();
   static_assert(smem + 640 <= 227 * 1024, "shared memory");
@@ -790,8 +804,11 @@ int launch_tc(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
 
 template <int HD>
 int tc_attention(Args& a, int q_heads, int max_nodes, cudaStream_t s) {
-  return max_nodes > 128 / a.rows.group ? launch_tc<HD, 2>(a, q_heads, max_nodes, s)
-                                        : launch_tc<HD, 1>(a, q_heads, max_nodes, s);
+  // (64 nodes of 4 heads over 16384 tokens, 12 requests: 209 us; with one stream per
+  // CTA, which reads each K/V tile once per 128 rows, 285.  The other way round, 64
+  // trees of 5 to 26 nodes: 68 us on two streams, of which one has no rows, 54 on one.)
+  return max_nodes > 128 / a.rows.group ? launch_tc<HD, 2>(a, q_heads, s)
+                                        : launch_tc<HD, 1>(a, q_heads, s);
 }
 
 // Node ancestors: bit m of node n's mask for m = n and every node on the way

@@ -306,3 +306,9 @@ def test_refusals_of_kept_buffers():
                 torch.zeros(3, dtype=torch.int64, device="cuda")):
         with pytest.raises(ValueError):
             pse.TokenTrees(c.trees.masks, c.nodes, offsets=bad)
+
+
+@pytest.mark.parametrize("group,nodes", [(17, [1]), (32, [1, 1]), (64, [2, 0, 1]), (2, [16, 3]), (2, [17, 16])])
+def test_few_rows_of_large_groups(group, nodes):
+    """The CUDA-core kernel's blocks hold whole groups, and any number of rows around its two sizes."""
+    Case([70] * len(nodes), nodes, 2 * group, 2, 40, 8, torch.float32, group).check()
