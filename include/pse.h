@@ -398,19 +398,21 @@ typedef struct {
   int32_t heads;
 } pse_head_view;
 
-/* q -> q_out and k -> k_out (either may have 0 heads); out may be the input
- * itself, but must not overlap it otherwise. */
-int pse_rotary(pse_rotary_spec r, pse_head_view q, pse_head_view q_out, pse_head_view k, pse_head_view k_out,
-               const int32_t *positions, int64_t tokens, int32_t dtype, void *stream);
+/* views: host array {q, q_out, k, k_out}, read before the call returns.  q -> q_out
+ * and k -> k_out (either may have 0 heads); out may be the input itself, but must
+ * not overlap it otherwise. */
+int pse_rotary(pse_rotary_spec r, const pse_head_view *views, const int32_t *positions, int64_t tokens,
+               int32_t dtype, void *stream);
 
 /* pse_rotary with the copy half of PagedKVCache.append
  * (engine/paged_cache.py:131-136): token t's turned K and its V also go to
  * position cache_pos[t] of slot slots[t] (blocks reserved before; a token
- * whose block is not held is dropped, as pse_kv_append drops it).  k_out.data
- * may be NULL.  The tensors have the pool's dtype. */
-int pse_rotary_append(pse_block_state st, pse_kv_layer kv, pse_rotary_spec r, pse_head_view q, pse_head_view q_out,
-                      pse_head_view k, pse_head_view k_out, pse_head_view v, const int32_t *positions,
-                      const int32_t *slots, const int32_t *cache_pos, int64_t tokens, void *stream);
+ * whose block is not held is dropped, as pse_kv_append drops it).  views: host
+ * array {q, q_out, k, k_out, v}; k_out.data may be NULL.  The tensors have the
+ * pool's dtype. */
+int pse_rotary_append(pse_block_state st, pse_kv_layer kv, pse_rotary_spec r, const pse_head_view *views,
+                      const int32_t *positions, const int32_t *slots, const int32_t *cache_pos, int64_t tokens,
+                      void *stream);
 
 /* ---- attention over packed prompts ---- */
 
@@ -425,7 +427,7 @@ int pse_prompt_plan(const int32_t *lens, int32_t n, int32_t q_heads, int32_t kv_
                     int64_t plan_ints, int64_t *n_ints);
 
 /* Causal attention of packed prompts (engine/model.py:99-116 without padding):
- * q, k, v and out are [tokens, heads, head_dim], prompt after prompt as planned;
+ * views: host array {q, k, v, out}, prompt after prompt as planned;
  * token i of a prompt attends to tokens 0..i of that prompt, query head h to K/V
  * head h / (q.heads / k.heads); head_dim <= 256.  A row whose weights sum to
  * zero gives zero.  bf16 with head_dim 64 or 128, at most 128 heads a group and
@@ -433,9 +435,8 @@ int pse_prompt_plan(const int32_t *lens, int32_t n, int32_t q_heads, int32_t kv_
  * cores.  Items that lie outside the tensors are skipped.  `status` (nullable)
  * receives PSE_STATUS_TIMEOUT if a bounded in-kernel wait expires.  `plan` is
  * the device copy of pse_prompt_plan's list. */
-int pse_prompt_attention(pse_head_view q, pse_head_view k, pse_head_view v, pse_head_view out, int64_t tokens,
-                         int32_t head_dim, int32_t dtype, float scale, const int32_t *plan, int32_t n_cta,
-                         int64_t n_items, int32_t *status, void *stream);
+int pse_prompt_attention(const pse_head_view *views, int64_t tokens, int32_t head_dim, int32_t dtype, float scale,
+                         const int32_t *plan, int32_t n_cta, int64_t n_items, int32_t *status, void *stream);
 
 /* ---- attention of token trees of any shape ---- */
 
@@ -448,23 +449,24 @@ int pse_tree_masks(const int32_t *parents, const int32_t *node_off, int32_t rows
                    int64_t *masks, int32_t *depths, void *stream);
 
 /* pse_paged_attention for token trees of any shape, ragged over the rows (the
- * reference lists trees as future work).  Row i's nodes are the queries
- * node_off[i]..node_off[i+1]-1 of q and out ([n_nodes, heads, head_dim]); node
+ * reference lists trees as future work).  views: host array {q, out}.  Row i's
+ * nodes are their tokens node_off[i]..node_off[i+1]-1 (n_nodes in all); node
  * j's K/V stands in the pool at position ctx[i] + j of slots[i].  Node j
  * attends to positions 0..ctx[i]-1 and to the row's nodes m whose bit is set in
  * its mask (`words` 64-bit words per node; bits past the row's nodes are
  * ignored, and a node need not see itself).  A node that sees nothing gives
  * zero, as do the nodes of a row with an invalid slot or a context the block
  * table cannot hold.  max_nodes bounds the rows' node counts (max_nodes <= 64
- * words; a row with more is left out, its output unwritten).  ctx, slots and node_off are read on
- * the device only, so the call can be captured and replayed with other values.
+ * words; a row with more is left out, its output unwritten).  ctx, slots and
+ * node_off are read on the device only, so the call can be captured and replayed
+ * with other values.
  * workspace: pse_token_tree_workspace() bytes, 16-byte aligned, written before
  * it is read (what stands in it does not matter); calls that share one must
  * not overlap on the GPU. */
-int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,
-                             const int32_t *slots, const int32_t *ctx, const int32_t *node_off, int32_t rows,
-                             int32_t n_nodes, int32_t max_nodes, const int64_t *masks, int32_t words, float scale,
-                             void *workspace, size_t workspace_bytes, void *stream);
+int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, const pse_head_view *views, const int32_t *slots,
+                             const int32_t *ctx, const int32_t *node_off, int32_t rows, int32_t n_nodes,
+                             int32_t max_nodes, const int64_t *masks, int32_t words, float scale, void *workspace,
+                             size_t workspace_bytes, void *stream);
 
 size_t pse_token_tree_workspace(int32_t head_dim);
 

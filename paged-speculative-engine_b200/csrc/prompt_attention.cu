@@ -636,9 +636,11 @@ extern "C" int pse_prompt_plan(const int32_t* lens, int32_t n, int32_t q_heads, 
   }
 }
 
-extern "C" int pse_prompt_attention(pse_head_view q, pse_head_view k, pse_head_view v, pse_head_view out,
-                                    int64_t tokens, int32_t head_dim, int32_t dtype, float scale, const int32_t* plan,
-                                    int32_t n_cta, int64_t n_items, int32_t* status, void* stream) {
+extern "C" int pse_prompt_attention(const pse_head_view* views, int64_t tokens, int32_t head_dim, int32_t dtype,
+                                    float scale, const int32_t* plan, int32_t n_cta, int64_t n_items, int32_t* status,
+                                    void* stream) {
+  if (!views) return PSE_EINVAL;
+  const pse_head_view &q = views[0], &k = views[1], &v = views[2], &out = views[3];
   if (tokens < 0 || tokens > 0x7fffffffll || head_dim <= 0 || head_dim > 256 || n_cta <= 0 || n_items < 0 ||
       n_items > 0x1fffffffll || (dtype != PSE_F32 && dtype != PSE_BF16) || q.heads <= 0 || k.heads <= 0 ||
       q.heads % k.heads || v.heads != k.heads || out.heads != q.heads)

@@ -259,8 +259,10 @@ int fill(RotaryArgs& a, const pse_rotary_spec& r, const pse_head_view& q, const 
 
 using namespace pse;
 
-extern "C" int pse_rotary(pse_rotary_spec r, pse_head_view q, pse_head_view q_out, pse_head_view k,
-                          pse_head_view k_out, const int32_t* positions, int64_t tokens, int32_t dtype, void* stream) {
+extern "C" int pse_rotary(pse_rotary_spec r, const pse_head_view* views, const int32_t* positions, int64_t tokens,
+                          int32_t dtype, void* stream) {
+  if (!views) return PSE_EINVAL;
+  const pse_head_view &q = views[0], &q_out = views[1], &k = views[2], &k_out = views[3];
   RotaryArgs a{};
   const int rc = fill(a, r, q, q_out, k, k_out, positions, tokens);
   if (rc != PSE_OK) return rc;
@@ -271,10 +273,11 @@ extern "C" int pse_rotary(pse_rotary_spec r, pse_head_view q, pse_head_view q_ou
                            : dispatch<float, false>(a, (cudaStream_t)stream);
 }
 
-extern "C" int pse_rotary_append(pse_block_state st, pse_kv_layer kv, pse_rotary_spec r, pse_head_view q,
-                                 pse_head_view q_out, pse_head_view k, pse_head_view k_out, pse_head_view v,
+extern "C" int pse_rotary_append(pse_block_state st, pse_kv_layer kv, pse_rotary_spec r, const pse_head_view* views,
                                  const int32_t* positions, const int32_t* slots, const int32_t* cache_pos,
                                  int64_t tokens, void* stream) {
+  if (!views) return PSE_EINVAL;
+  const pse_head_view &q = views[0], &q_out = views[1], &k = views[2], &k_out = views[3], &v = views[4];
   RotaryArgs a{};
   const int rc = fill(a, r, q, q_out, k, k_out, positions, tokens);
   if (rc != PSE_OK) return rc;

@@ -857,11 +857,13 @@ extern "C" size_t pse_token_tree_workspace(int32_t head_dim) {
   return tree::kCutBytes + (head_dim <= 128 && tc > simt ? tc : simt) * 2 * tree::part_width(head_dim) * 4;
 }
 
-extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, pse_head_view q, pse_head_view out,
+extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, const pse_head_view* views,
                                         const int32_t* slots, const int32_t* ctx, const int32_t* node_off,
                                         int32_t rows, int32_t n_nodes, int32_t max_nodes, const int64_t* masks,
                                         int32_t words, float scale, void* workspace, size_t workspace_bytes,
                                         void* stream) {
+  if (!views) return PSE_EINVAL;
+  const pse_head_view &q = views[0], &out = views[1];
   if (!st.block_table || !st.nblocks || !st.status || st.block_size <= 0 || st.max_blocks <= 0 || st.num_slots <= 0 ||
       !kv.k_pool || !kv.v_pool || kv.kv_heads <= 0 || kv.head_dim <= 0 || kv.head_dim > 256 || rows < 0 ||
       n_nodes < 0 || max_nodes < 0 || words <= 0 || max_nodes > 64ll * words || q.heads <= 0 ||

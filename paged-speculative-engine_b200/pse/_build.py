@@ -12,8 +12,8 @@ CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 LIB = os.path.join(PKG, "lib", "libpse.so")
 
-SOURCES = ["kv_cache.cu", "attention.cu", "attention_tc.cu", "attention_prefill.cu", "gemm_tc.cu", "sampling.cu", "model_ops.cu", "sched.cu",
-           "rotary.cu", "prompt_attention.cu", "tree_attention.cu"]
+SOURCES = ["kv_cache.cu", "attention.cu", "attention_tc.cu", "attention_prefill.cu", "gemm_tc.cu", "sampling.cu",
+           "model_ops.cu", "sched.cu", "rotary.cu", "prompt_attention.cu", "tree_attention.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -11,6 +11,7 @@ import contextlib
 import ctypes
 import gc
 import os
+import struct
 import threading
 from collections import Counter
 
@@ -53,8 +54,13 @@ class RotarySpec(ctypes.Structure):
     _fields_ = [("turns", c_p), ("factor", c_f32), ("head_dim", c_i32), ("rotary_dim", c_i32), ("interleaved", c_i32)]
 
 
-class HeadView(ctypes.Structure):
-    _fields_ = [("data", c_p), ("tok_stride", c_i64), ("head_stride", c_i64), ("heads", c_i32)]
+def _views(n: int):
+    return struct.Struct("=" + "Qqqi4x" * n).pack
+
+
+# arrays of pse_head_view as bytes, from (data, tok_stride, head_stride, heads) each
+# (a ctypes structure per view costs a third of a small call's host time)
+views2, views4, views5 = _views(2), _views(4), _views(5)
 
 
 # name -> (argtypes, kernels launched per call)
@@ -87,15 +93,13 @@ _PROTOS = {
                       c_i32, c_p], 1),
     "pse_epilogue": ([c_i32, c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i32, c_i32, c_i32, c_p], 1),
     "pse_rope": ([c_p, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32, c_p, c_f32, c_i32, c_p], 1),
-    "pse_rotary": ([RotarySpec, HeadView, HeadView, HeadView, HeadView, c_p, c_i64, c_i32, c_p], 1),
-    "pse_rotary_append": ([BlockState, KVLayer, RotarySpec, HeadView, HeadView, HeadView, HeadView, HeadView, c_p, c_p,
-                           c_p, c_i64, c_p], 1),
+    "pse_rotary": ([RotarySpec, c_p, c_p, c_i64, c_i32, c_p], 1),
+    "pse_rotary_append": ([BlockState, KVLayer, RotarySpec, c_p, c_p, c_p, c_p, c_i64, c_p], 1),
     "pse_prompt_plan": ([c_p, c_i32, c_i32, c_i32, c_i32, c_p, c_i64, c_p], 0),
-    "pse_prompt_attention": ([HeadView, HeadView, HeadView, HeadView, c_i64, c_i32, c_i32, c_f32, c_p, c_i32, c_i64,
-                              c_p, c_p], 1),
+    "pse_prompt_attention": ([c_p, c_i64, c_i32, c_i32, c_f32, c_p, c_i32, c_i64, c_p, c_p], 1),
     "pse_tree_masks": ([c_p, c_p, c_i32, c_i32, c_i32, c_p, c_p, c_p], 1),
-    "pse_token_tree_attention": ([BlockState, KVLayer, HeadView, HeadView, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_p,
-                                  c_i32, c_f32, c_p, c_sz, c_p], 2),
+    "pse_token_tree_attention": ([BlockState, KVLayer, c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_p, c_i32, c_f32,
+                                  c_p, c_sz, c_p], 2),
     "pse_scatter_rows": ([c_p, c_i64, c_p, c_i32, c_i32, c_p, c_i64, c_i32, c_p], 1),
     "pse_attention_force_generic": ([c_i32], 0),
     "pse_accept_select": ([c_i32], 0),

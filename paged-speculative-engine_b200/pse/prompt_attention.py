@@ -85,7 +85,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompts:
         out, ov = new_result(q, qv, hd)
     else:
         ov = head_view("out", out, T, prompts.q_heads, hd, dtype, dev)
-    rc = prompts.fn(qv, kv, vv, ov, T, hd, code, 1.0 / math.sqrt(hd) if scale is None else float(scale),
+    rc = prompts.fn(N.views4(*qv, *kv, *vv, *ov), T, hd, code, 1.0 / math.sqrt(hd) if scale is None else float(scale),
                     prompts._plan_ptr, prompts.n_cta, prompts.n_items, prompts._status_ptr, N.stream_ptr())
     if rc:
         raise N.failed("pse_prompt_attention", rc)

@@ -109,11 +109,11 @@ class RotaryPlan:
                                  int(self.interleaved))
 
 
-_NO_HEADS = N.HeadView(None, 0, 0, 0)
+_NO_HEADS = (0, 0, 0, 0)
 
 
-def head_view(name: str, t: torch.Tensor, tokens, heads, head_dim: int, dtype, device: int) -> N.HeadView:
-    """The library's view of ``t``, which must be [tokens, heads, head_dim] with
+def head_view(name: str, t: torch.Tensor, tokens, heads, head_dim: int, dtype, device: int) -> tuple:
+    """The library's view of ``t`` (address, strides, heads), which must be [tokens, heads, head_dim] with
     a contiguous last axis, of ``dtype``, on GPU ``device`` (tokens or heads
     None: any)."""
     try:
@@ -128,7 +128,7 @@ def head_view(name: str, t: torch.Tensor, tokens, heads, head_dim: int, dtype, d
         raise ValueError(f"{name} must be {dtype} on GPU {device}, got {t.dtype} on {t.device}")
     if s2 != 1 and T * H * D:
         raise ValueError(f"{name}'s last axis must be contiguous")
-    return N.HeadView(t.data_ptr(), s0, s1, H)
+    return t.data_ptr(), s0, s1, H
 
 
 def index_ptr(name: str, t: torch.Tensor, n: int, device: int) -> int:
@@ -139,16 +139,16 @@ def index_ptr(name: str, t: torch.Tensor, n: int, device: int) -> int:
     return t.data_ptr()
 
 
-def new_result(src: torch.Tensor, view: N.HeadView, head_dim: int):
+def new_result(src: torch.Tensor, view: tuple, head_dim: int):
     """A contiguous result tensor of the shape of ``src`` ([tokens, heads,
     head_dim], checked as ``view``) and the library's view of it."""
-    out, heads = torch.empty_like(src, memory_format=torch.contiguous_format), view.heads
-    return out, N.HeadView(out.data_ptr(), heads * head_dim, head_dim, heads)
+    out, heads = torch.empty_like(src, memory_format=torch.contiguous_format), view[3]
+    return out, (out.data_ptr(), heads * head_dim, head_dim, heads)
 
 
-def _out_view(name: str, out: torch.Tensor, src: torch.Tensor, view: N.HeadView, head_dim: int, dtype, device: int):
-    v = head_view(name, out, src.shape[0], view.heads, head_dim, dtype, device)
-    if v.data == view.data and (v.tok_stride != view.tok_stride or v.head_stride != view.head_stride) and src.numel():
+def _out_view(name: str, out: torch.Tensor, src: torch.Tensor, view: tuple, head_dim: int, dtype, device: int):
+    v = head_view(name, out, src.shape[0], view[3], head_dim, dtype, device)
+    if v[0] == view[0] and v[1:3] != view[1:3] and src.numel():
         raise ValueError(f"{name} overlaps its input with other strides")
     return v
 
@@ -174,7 +174,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
             k_out, ko = new_result(k, kv, hd)
         else:
             ko = _out_view("k_out", k_out, k, kv, hd, dtype, dev)
-    rc = plan.fn(plan.spec, qv, qo, kv, ko, pos, T, code, N.stream_ptr())
+    rc = plan.fn(plan.spec, N.views4(*qv, *qo, *kv, *ko), pos, T, code, N.stream_ptr())
     if rc:
         raise N.failed("pse_rotary", rc)
     N.launches["pse_rotary"] += 1
@@ -207,7 +207,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     else:
         qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
     ko = _NO_HEADS if k_out is None else _out_view("k_out", k_out, k, kv, hd, dtype, dev)
-    rc = plan.append_fn(cache.state, cache.layer(layer), plan.spec, qv, qo, kv, ko, vv, pos, slot, at, T,
+    rc = plan.append_fn(cache.state, cache.layer(layer), plan.spec, N.views5(*qv, *qo, *kv, *ko, *vv), pos, slot, at, T,
                         N.stream_ptr())
     if rc:
         raise N.failed("pse_rotary_append", rc)

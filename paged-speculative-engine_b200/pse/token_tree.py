@@ -105,7 +105,7 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
     if not 0 <= layer < cache.n_layers:
         raise ValueError(f"layer {layer} of a cache with {cache.n_layers}")
     qv = head_view("q", q, trees.nodes, None, hd, dtype, dev)
-    heads, rows = qv.heads, len(trees.counts)
+    heads, rows = qv[3], len(trees.counts)
     if heads == 0 or heads % cache.n_heads or heads // cache.n_heads > 64 or hd > 256:
         raise ValueError(f"{heads} query heads over {cache.n_heads} K/V heads of {hd}")
     slot, ctx = index_ptr("slots", slots, rows, dev), index_ptr("context", context, rows, dev)
@@ -117,7 +117,7 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
         workspace = token_tree_workspace(hd, q.device)
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError(f"workspace must be a contiguous uint8 tensor on GPU {dev}")
-    rc = trees.fn(cache.state, cache.layer(layer), qv, ov, slot, ctx, trees._offsets_ptr, rows, trees.nodes,
+    rc = trees.fn(cache.state, cache.layer(layer), N.views2(*qv, *ov), slot, ctx, trees._offsets_ptr, rows, trees.nodes,
                   trees.max_nodes, trees._masks_ptr, trees.words, 1.0 / math.sqrt(hd) if scale is None else float(scale),
                   workspace.data_ptr(), workspace.numel(), N.stream_ptr())
     if rc:
