@@ -390,6 +390,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (more) mma_commit(el, &slot_empty[k]);
           if (j + 2 == n) mma_commit(el, q_empty);
         }
+        // a stream that has no part in this item holds nothing up above: however
+        // many such items follow, its output of an earlier one is read (and that
+        // item's word in `poison` with it) before this warp goes on
+        if (n1 == 0 && run) run = mbar_wait_warp(&o_empty[1], outs >> 1 & 1u, vabort);
       }
       mma_commit(el, final_bar);
     } else if (warp == 10) {

@@ -211,3 +211,24 @@ def test_refusals():
     for a in (([-1], 4, 2), ([3], 4, 3), ([3], 0, 1), ([1 << 30, 1 << 30], 4, 2)):
         with pytest.raises(ValueError):
             pse.PackedPrompts(*a)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_short_items_behind_a_long_one(hd):
+    """Every multiprocessor takes items of two query tiles and then many of one,
+    whose second stream has no part in them; the marks of value tiles with
+    infinities stay with their own item."""
+    lens = [200] * 20 + [100] * 260 + [1] * 40
+    hq = hk = 8
+    q, k, v = (x.clone() for x in inputs(lens, hq, hk, hd, torch.bfloat16, 21))
+    clean = run(q, k, v, lens)
+    check(q, k, v, lens)
+    seen, t = torch.zeros_like(clean, dtype=torch.bool), 0
+    for i, n in enumerate(lens):
+        at = t + n * 3 // 4  # in the second tile of a long prompt
+        if i % 3 == 0:
+            v[at, i % hk, i % hd] = math.inf
+            seen[at:t + n, i % hk, i % hd] = True
+        t += n
+    got = run(q, k, v, lens)
+    assert bool((got[seen] == math.inf).all()) and torch.equal(got[~seen], clean[~seen])
