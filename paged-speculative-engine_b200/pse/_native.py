@@ -168,6 +168,17 @@ def stream_ptr() -> int:
     return _raw_stream(_current_device())
 
 
+def stream_on(index: int) -> int:
+    """``stream_ptr`` for a launch over memory of GPU ``index``.  Kernels launch on
+    the current device, which has to be that one: another GPU's addresses are no
+    addresses there."""
+    current = torch.cuda.current_device() if _current_device is None else _current_device()
+    if current != index:
+        raise ValueError(f"the tensors are on GPU {index} and GPU {current} is current: "
+                         f"make the call under torch.cuda.device({index})")
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(index)
+
+
 def call(name: str, *args) -> None:
     lib = _lib if _lib is not None else load()
     rc = getattr(lib, name)(*args)

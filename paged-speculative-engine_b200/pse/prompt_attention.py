@@ -17,8 +17,8 @@ class PackedPrompts:
     """The packing of one batch of prompts: ``lengths`` tokens each, one after
     the other, and the attention's work list for it (built on the host, one
     copy to the device).  One object serves every layer of a forward and any
-    number of calls; it is not changed by them, except for ``status``, where a
-    kernel leaves an error (``check_status``)."""
+    number of calls, made with its device current; it is not changed by them,
+    except for ``status``, where a kernel leaves an error (``check_status``)."""
 
     def __init__(self, lengths, q_heads: int, kv_heads: int, device=None) -> None:
         N.load()
@@ -73,6 +73,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompts:
     [T, q_heads, head_dim] (``out`` if given, which must not overlap the
     inputs)."""
     shape, dtype, dev = getattr(q, "shape", ()), getattr(q, "dtype", None), prompts.index
+    stream = N.stream_on(dev)
     hd = shape[2] if len(shape) == 3 else 0
     if not 0 < hd <= 256:
         raise ValueError(f"q must be [tokens, heads, head_dim] with a head_dim of 1 to 256, got {tuple(shape)}")
@@ -86,7 +87,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompts:
     else:
         ov = head_view("out", out, T, prompts.q_heads, hd, dtype, dev)
     rc = prompts.fn(N.views4(*qv, *kv, *vv, *ov), T, hd, code, 1.0 / math.sqrt(hd) if scale is None else float(scale),
-                    prompts._plan_ptr, prompts.n_cta, prompts.n_items, prompts._status_ptr, N.stream_ptr())
+                    prompts._plan_ptr, prompts.n_cta, prompts.n_items, prompts._status_ptr, stream)
     if rc:
         raise N.failed("pse_prompt_attention", rc)
     N.launches["pse_prompt_attention"] += 1

@@ -88,7 +88,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
 class RotaryPlan:
     """A model's rotary positions: frequencies in turns per position on the
     device (fp64, ``rotary_dim / 2`` entries), the pair layout and the factor.
-    Build it once per model and device; it holds no state between calls."""
+    Build it once per model and device; it holds no state between calls, which
+    are made with that device current."""
 
     def __init__(self, head_dim: int, *, rotary_dim: int | None = None, theta: float = 10000.0,
                  interleaved: bool = False, scaling: dict | None = None, device=None) -> None:
@@ -160,6 +161,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
     a fused projection included).  Results go to ``q_out`` / ``k_out`` (which
     may be q / k themselves) or to new tensors, and are returned as (q, k)."""
     hd, dev, dtype = plan.head_dim, plan.index, getattr(q, "dtype", None)
+    stream = N.stream_on(dev)
     qv = head_view("q", q, None, None, hd, dtype, dev)
     code, T = N.dtype_code(dtype), q.shape[0]
     pos = index_ptr("positions", positions, T, dev)
@@ -174,7 +176,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, pla
             k_out, ko = new_result(k, kv, hd)
         else:
             ko = _out_view("k_out", k_out, k, kv, hd, dtype, dev)
-    rc = plan.fn(plan.spec, N.views4(*qv, *qo, *kv, *ko), pos, T, code, N.stream_ptr())
+    rc = plan.fn(plan.spec, N.views4(*qv, *qo, *kv, *ko), pos, T, code, stream)
     if rc:
         raise N.failed("pse_rotary", rc)
     N.launches["pse_rotary"] += 1
@@ -191,6 +193,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     from the cache's for tree nodes.  ``k_out``, if given, receives the turned
     k as well.  Returns the turned q."""
     hd, dev, dtype = plan.head_dim, plan.index, cache.dtype
+    stream = N.stream_on(dev)
     if cache.head_dim != hd or cache.device.index != dev:
         raise ValueError("the cache and the plan must match in head_dim and device")
     if not 0 <= layer < cache.n_layers:
@@ -208,7 +211,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         qo = _out_view("q_out", q_out, q, qv, hd, dtype, dev)
     ko = _NO_HEADS if k_out is None else _out_view("k_out", k_out, k, kv, hd, dtype, dev)
     rc = plan.append_fn(cache.state, cache.layer(layer), plan.spec, N.views5(*qv, *qo, *kv, *ko, *vv), pos, slot, at, T,
-                        N.stream_ptr())
+                        stream)
     if rc:
         raise N.failed("pse_rotary_append", rc)
     N.launches["pse_rotary_append"] += 1

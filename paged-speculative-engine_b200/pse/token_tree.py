@@ -67,6 +67,7 @@ def tree_masks(parents: torch.Tensor, counts) -> TokenTrees:
     n = sum(counts)
     if not torch.is_tensor(parents) or not parents.is_cuda:
         raise ValueError("parents must be on a GPU")
+    stream = N.stream_on(parents.get_device())
     index_ptr("parents", parents, n, parents.get_device())
     words = max(1, (max(counts, default=0) + 63) // 64)
     offsets = _offsets(counts, parents.device)
@@ -74,7 +75,7 @@ def tree_masks(parents: torch.Tensor, counts) -> TokenTrees:
     depths = torch.empty(n, dtype=torch.int32, device=parents.device)
     trees = TokenTrees(masks, counts, depths, offsets)
     N.call("pse_tree_masks", parents.data_ptr(), offsets.data_ptr(), len(counts), n, words, masks.data_ptr(),
-           depths.data_ptr(), N.stream_ptr())
+           depths.data_ptr(), stream)
     return trees
 
 
@@ -100,6 +101,7 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
     j at position context + j.  ``scale`` defaults to 1 / sqrt(head_dim).
     Returns [nodes, q_heads, head_dim]; a node that sees nothing gives zeros."""
     hd, dtype, dev = cache.head_dim, cache.dtype, trees.index
+    stream = N.stream_on(dev)
     if cache.device.index != dev:
         raise ValueError("the cache and the trees must be on one device")
     if not 0 <= layer < cache.n_layers:
@@ -119,7 +121,7 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
         raise ValueError(f"workspace must be a contiguous uint8 tensor on GPU {dev}")
     rc = trees.fn(cache.state, cache.layer(layer), N.views2(*qv, *ov), slot, ctx, trees._offsets_ptr, rows, trees.nodes,
                   trees.max_nodes, trees._masks_ptr, trees.words, 1.0 / math.sqrt(hd) if scale is None else float(scale),
-                  workspace.data_ptr(), workspace.numel(), N.stream_ptr())
+                  workspace.data_ptr(), workspace.numel(), stream)
     if rc:
         raise N.failed("pse_token_tree_attention", rc)
     N.launches["pse_token_tree_attention"] += 2
