@@ -173,7 +173,9 @@ class PagedKVCache:
         self.block_size, self.num_blocks = block_size, num_blocks
         self.dtype = dtype
         self.dtype_code = N.dtype_code(dtype)
-        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.device = torch.device("cuda" if device is None else device)
+        if self.device.type == "cuda" and self.device.index is None:  # "cuda" is the current one
+            self.device = torch.device("cuda", torch.cuda.current_device())
         shape = (n_layers, num_blocks, n_heads, block_size, head_dim)
         self.k_pool = torch.zeros(shape, dtype=dtype, device=self.device)
         self.v_pool = torch.zeros(shape, dtype=dtype, device=self.device)
