@@ -36,8 +36,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
       between blend linearly in their number of turns.
     * ``yarn`` (``factor``, ``original``, ``fast``, ``slow``): the same idea
       with the blend linear in the pair's index, between the indices that turn
-      ``fast`` and ``slow`` times, and a factor 0.1 ln(factor) + 1 on sine and
-      cosine (``attention_factor`` overrides it).
+      ``fast`` and ``slow`` times, and a factor 0.1 ln(factor) + 1, but at
+      least 1, on sine and cosine (``attention_factor`` overrides it).
     """
     if rotary_dim < 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even, got {rotary_dim}")
@@ -82,7 +82,7 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
     for i, x in enumerate(f):
         blend = min(1.0, max(0.0, (i - first) / max(last - first, 0.001)))
         out.append((1.0 - blend) * x + blend * (x / factor))
-    return out, _number(scaling, "attention_factor", 0.1 * math.log(factor) + 1.0)
+    return out, _number(scaling, "attention_factor", 0.1 * math.log(max(factor, 1.0)) + 1.0)
 
 
 class RotaryPlan:

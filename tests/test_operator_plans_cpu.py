@@ -96,3 +96,11 @@ def test_frequency_refusals(bad):
     from pse import rotary_frequencies
     with pytest.raises(ValueError):
         rotary_frequencies(64, scaling=bad)
+
+
+@pytest.mark.parametrize("factor,want", [(1.0, 1.0), (0.5, 1.0), (1e-6, 1.0), (2.0, 0.1 * math.log(2.0) + 1.0)])
+def test_yarn_does_not_flatten_the_logits_of_shortened_contexts(factor, want):
+    """The temperature belongs to contexts that grew; below a factor of 1 it stays 1."""
+    from pse import rotary_frequencies
+    f, got = rotary_frequencies(64, scaling={"type": "yarn", "factor": factor, "original": 4096})
+    assert math.isclose(got, want, rel_tol=1e-15) and math.isclose(f[31] * factor, 10000.0 ** (-62 / 64), rel_tol=1e-12)
