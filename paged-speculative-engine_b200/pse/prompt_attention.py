@@ -10,7 +10,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from .rotary import head_view, new_result
+from .rotary import head_view, new_result, written_view
 
 
 class PackedPrompts:
@@ -85,7 +85,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompts:
     if out is None:
         out, ov = new_result(q, qv, hd)
     else:
-        ov = head_view("out", out, T, prompts.q_heads, hd, dtype, dev)
+        ov = written_view("out", out, T, prompts.q_heads, hd, dtype, dev)
     rc = prompts.fn(N.views4(*qv, *kv, *vv, *ov), T, hd, code, 1.0 / math.sqrt(hd) if scale is None else float(scale),
                     prompts._plan_ptr, prompts.n_cta, prompts.n_items, prompts._status_ptr, stream)
     if rc:

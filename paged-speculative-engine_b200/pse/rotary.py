@@ -132,6 +132,18 @@ def head_view(name: str, t: torch.Tensor, tokens, heads, head_dim: int, dtype, d
     return t.data_ptr(), s0, s1, H
 
 
+def written_view(name: str, t: torch.Tensor, tokens: int, heads: int, head_dim: int, dtype, device: int) -> tuple:
+    """``head_view`` of a tensor that the kernel writes, whose elements must each
+    have a place of their own."""
+    view = head_view(name, t, tokens, heads, head_dim, dtype, device)
+    reach = head_dim
+    for stride, n in sorted(((view[1], tokens), (view[2], heads))):
+        if n > 1 and stride < reach and tokens and heads:
+            raise ValueError(f"{name} overlaps itself (strides {t.stride()})")
+        reach += max(n - 1, 0) * stride
+    return view
+
+
 def index_ptr(name: str, t: torch.Tensor, n: int, device: int) -> int:
     """The address of ``t``, a contiguous int32 tensor of n entries on GPU ``device``."""
     if not torch.is_tensor(t) or t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or \
@@ -148,7 +160,7 @@ def new_result(src: torch.Tensor, view: tuple, head_dim: int):
 
 
 def _out_view(name: str, out: torch.Tensor, src: torch.Tensor, view: tuple, head_dim: int, dtype, device: int):
-    v = head_view(name, out, src.shape[0], view[3], head_dim, dtype, device)
+    v = written_view(name, out, src.shape[0], view[3], head_dim, dtype, device)
     if v[0] == view[0] and v[1:3] != view[1:3] and src.numel():
         raise ValueError(f"{name} overlaps its input with other strides")
     return v

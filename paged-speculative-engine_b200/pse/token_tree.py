@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _native as N
-from .rotary import head_view, index_ptr, new_result
+from .rotary import head_view, index_ptr, new_result, written_view
 
 MAX_NODES = 4096  # nodes of one request's tree
 
@@ -114,7 +114,7 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
     if out is None:
         out, ov = new_result(q, qv, hd)
     else:
-        ov = head_view("out", out, trees.nodes, heads, hd, dtype, dev)
+        ov = written_view("out", out, trees.nodes, heads, hd, dtype, dev)
     if workspace is None:
         workspace = token_tree_workspace(hd, q.device)
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != dev or not workspace.is_contiguous():
