@@ -15,6 +15,7 @@
 
 #include "attention_tile.cuh"
 #include "simt_attention.cuh"
+#include "tmap_cache.h"
 
 namespace pse {
 namespace prompt {
@@ -554,9 +555,9 @@ int launch_tc(const Args& a, cudaStream_t s) {
                    (uint64_t)(heads == 1 ? HD : head) * 2, (uint64_t)tok * 2, b1, b2};
   };
   CUtensorMap mq, mk, mv;
-  int rc = g_maps.get(key(a.q, a.q_tok, a.q_head, a.q_heads, a.group, tile_tokens(a.group)), &mq);
-  if (rc == 0) rc = g_maps.get(key(a.k, a.k_tok, a.k_head, a.kv_heads, 1, 128), &mk);
-  if (rc == 0) rc = g_maps.get(key(a.v, a.v_tok, a.v_head, a.kv_heads, 1, 128), &mv);
+  int rc = g_maps.get(key(a.q, a.q_tok, a.q_head, a.q_heads, a.group, tile_tokens(a.group)), PSE_EINVAL, &mq);
+  if (rc == 0) rc = g_maps.get(key(a.k, a.k_tok, a.k_head, a.kv_heads, 1, 128), PSE_EINVAL, &mk);
+  if (rc == 0) rc = g_maps.get(key(a.v, a.v_tok, a.v_head, a.kv_heads, 1, 128), PSE_EINVAL, &mv);
   if (rc) return rc;
   // with fewer items than CTAs the plan gives them to the first ones
   const int grid = a.n_items < a.n_cta ? a.n_items : a.n_cta;

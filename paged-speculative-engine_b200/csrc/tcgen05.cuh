@@ -4,10 +4,6 @@
 #pragma once
 
 #include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <mutex>
-#include <unordered_map>
 
 #include "common.cuh"
 
@@ -290,64 +286,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-
-// ---------------------------------------------------------------- tensor maps
-// [d2, d1, d0] bf16 with strides s2, s1 (bytes), boxes of [b2, b1, 64], 128-byte
-// swizzle, elements out of range read as zero.  A map is a pure function of
-// the key, every field of which is compared on a hit; the cache is bounded.
-struct Map3Key {
-  uint64_t ptr, d0, d1, d2, s1, s2;
-  uint32_t b1, b2;
-  bool operator==(const Map3Key& o) const {
-    return ptr == o.ptr && d0 == o.d0 && d1 == o.d1 && d2 == o.d2 && s1 == o.s1 && s2 == o.s2 && b1 == o.b1 &&
-           b2 == o.b2;
-  }
-};
-struct Map3Hash {
-  size_t operator()(const Map3Key& k) const {
-    uint64_t h = 1469598103934665603ull;
-    for (uint64_t v : {k.ptr, k.d0, k.d1, k.d2, k.s1, k.s2, (uint64_t)k.b1, (uint64_t)k.b2})
-      h = (h ^ v) * 1099511628211ull;
-    return (size_t)h;
-  }
-};
-class Map3Cache {
- public:
-  static constexpr size_t kMaxEntries = 4096;
-  int get(const Map3Key& key, CUtensorMap* out) {
-    std::lock_guard<std::mutex> lk(mu_);
-    auto it = maps_.find(key);
-    if (it != maps_.end()) {
-      *out = it->second;
-      return 0;
-    }
-    if (!encode_) {
-      cudaDriverEntryPointQueryResult q;
-      void* fn = nullptr;
-      const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-      if (e != cudaSuccess) return (int)e;
-      if (q != cudaDriverEntryPointSuccess || !fn) return PSE_EINVAL;
-      encode_ = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    CUtensorMap m;
-    const cuuint64_t dims[3] = {key.d0, key.d1, key.d2};
-    const cuuint64_t strides[2] = {key.s1, key.s2};
-    const cuuint32_t box[3] = {64u, key.b1, key.b2}, estr[3] = {1, 1, 1};
-    if (encode_(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, reinterpret_cast<void*>(key.ptr), dims, strides, box, estr,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return PSE_EINVAL;
-    if (maps_.size() >= kMaxEntries) maps_.clear();
-    maps_.emplace(key, m);
-    *out = m;
-    return 0;
-  }
-
- private:
-  std::mutex mu_;
-  PFN_cuTensorMapEncodeTiled_v12000 encode_ = nullptr;
-  std::unordered_map<Map3Key, CUtensorMap, Map3Hash> maps_;
-};
 
 }  // namespace t5
 }  // namespace pse

@@ -790,7 +790,7 @@ int launch_tc(Args& a, int q_heads, cudaStream_t s) {
   int rc = g_q_maps.get(Map3Key{reinterpret_cast<uint64_t>(a.q), (uint64_t)HD, (uint64_t)q_heads,
                                 (uint64_t)a.rows.n_nodes, (uint64_t)(q_heads == 1 ? HD : a.q_head) * 2,
                                 (uint64_t)a.q_tok * 2, (uint32_t)a.rows.group, (uint32_t)tpt},
-                        &mq);
+                        PSE_EINVAL, &mq);
   const uint64_t pool_rows = (uint64_t)a.num_blocks * a.rows.kv_heads * a.block_size;
   if (rc == 0) rc = g_pool_maps.get(a.k_pool, HD, pool_rows, HD * 2, 64u, a.block_size, PSE_EINVAL, &mk);
   if (rc == 0) rc = g_pool_maps.get(a.v_pool, HD, pool_rows, HD * 2, 64u, a.block_size, PSE_EINVAL, &mv);
