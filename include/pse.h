@@ -438,6 +438,14 @@ int pse_prompt_plan(const int32_t *lens, int32_t n, int32_t q_heads, int32_t kv_
 int pse_prompt_attention(const pse_head_view *views, int64_t tokens, int32_t head_dim, int32_t dtype, float scale,
                          const int32_t *plan, int32_t n_cta, int64_t n_items, int32_t *status, void *stream);
 
+/* Tries that the tensor-core products' bounded waits may take (token trees: those
+ * for a piece of work's first copies) in launches of pse_prompt_attention and
+ * pse_token_tree_attention from now on: a few microseconds each; negative: the
+ * default of 2^18; 0: none.  For tests of what follows an expired wait: the
+ * kernel lets its copies and products in flight end, sets PSE_STATUS_TIMEOUT and
+ * returns, its output incomplete. */
+int pse_attention_wait_tries(int32_t tries);
+
 /* ---- attention of token trees of any shape ---- */
 
 /* Ancestor masks and depths of packed trees: parents[node_off[i] + j] is the

@@ -10,6 +10,7 @@
 // far, which needs no counter on the device and gives the same order of
 // operations in every call.
 #include <algorithm>
+#include <atomic>
 #include <queue>
 #include <vector>
 
@@ -18,6 +19,14 @@
 #include "tmap_cache.h"
 
 namespace pse {
+
+namespace t5 {
+namespace {
+std::atomic<uint32_t> g_wait_tries{kSpinLimit};
+}
+uint32_t wait_tries() { return g_wait_tries.load(std::memory_order_relaxed); }
+}  // namespace t5
+
 namespace prompt {
 
 struct Args {
@@ -31,6 +40,7 @@ struct Args {
   int n_cta, n_items;
   int32_t* status;
   bool out_vec;  // output rows are 16-byte aligned
+  uint32_t wait_tries;  // of the products
 };
 
 // Tokens of one query tile: at most 128 rows of (token, group head).
@@ -224,7 +234,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   int* poison = abort_flag + 1;            // [kGuards] items' marked tiles, bit j: tile guard0 + j
   int* last_bar = poison + kGuards;        // [NS + 1] per slot (and Q): barrier and parity of its last copy
-  volatile int* vabort = abort_flag;
+  const Waits waits{abort_flag, kSpinLimit};
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
@@ -273,7 +283,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bool run = true;
         auto load = [&](const CUtensorMap* map, int hk, int tok, bool guarded) -> bool {
           const int s = c % NS;
-          if (!mbar_wait(&slot_empty[s], ((c / NS) & 1) ^ 1, vabort)) return false;
+          if (!mbar_wait(&slot_empty[s], ((c / NS) & 1) ^ 1, waits)) return false;
           uint64_t* bar = guarded ? &guard_full[g % kGuards] : &slot_full[s];
           last_bar[s] = guarded ? (NS + g % kGuards) * 2 + ((g / kGuards) & 1) : s * 2 + ((c / NS) & 1);
           mbar_expect_tx(bar, kTileBytes);
@@ -302,7 +312,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int e = e0; e < e1; ++e) {
           const TcItem it = decode(a, e, tpt);
           if (it.n_max == 0) continue;
-          if (!mbar_wait(q_empty, (nq & 1) ^ 1, vabort)) break;
+          if (!mbar_wait(q_empty, (nq & 1) ^ 1, waits)) break;
           const int streams = it.n[1] > 0 ? 2 : 1;
           last_bar[NS] = nq & 1;
           mbar_expect_tx(q_full, streams * kHalves * tpt * a.group * 128);
@@ -318,6 +328,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (warp == 9) {
       // -------------------------------------------------------------- products
       const uint32_t el = elect_one();
+      const Waits tries{abort_flag, a.wait_tries};
       const uint32_t full0 = su32(slot_full), empty0 = su32(slot_empty), ring0 = su32(ring), q0 = su32(q_s);
       const uint32_t part0 = su32(p_half);
       int slot = 0;
@@ -341,7 +352,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int k, v = 0;
         uint32_t kp, vp = 0;
         next_slot(k, kp);
-        run = mbar_wait3_warp(su32(q_full), nq, full0 + 8 * k, kp, full0 + 8 * k, kp, vabort);
+        run = mbar_wait3_warp(su32(q_full), nq, full0 + 8 * k, kp, full0 + 8 * k, kp, tries);
         nq ^= 1;
         if (!run) break;
         fence_after();
@@ -365,13 +376,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (j >= ns || !run) return;
             const uint32_t s_col = tmem + kColS + s * 128, o_col = tmem + kColO + s * 128, part = part0 + 16 * s;
             const uint32_t np = parts >> s & 1u;
-            if (j == 0) run = mbar_wait_warp(&o_empty[s], outs >> s & 1u, vabort);
-            run = run && (here ? mbar_wait_warp(part, np, vabort) : mbar_wait3_warp(part, np, vbar, vp, kbar, kp, vabort));
+            if (j == 0) run = mbar_wait_warp(&o_empty[s], outs >> s & 1u, tries);
+            run = run && (here ? mbar_wait_warp(part, np, tries) : mbar_wait3_warp(part, np, vbar, vp, kbar, kp, tries));
             here = true;
             if (!run) return;
             fence_after();
             issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 0, j == 0);
-            run = mbar_wait_warp(part + 8, np, vabort);
+            run = mbar_wait_warp(part + 8, np, tries);
             if (!run) return;
             fence_after();
             issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 1, false);
@@ -394,7 +405,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // a stream that has no part in this item holds nothing up above: however
         // many such items follow, its output of an earlier one is read (and that
         // item's word in `poison` with it) before this warp goes on
-        if (n1 == 0 && run) run = mbar_wait_warp(&o_empty[1], outs >> 1 & 1u, vabort);
+        if (n1 == 0 && run) run = mbar_wait_warp(&o_empty[1], outs >> 1 & 1u, tries);
       }
       mma_commit(el, final_bar);
     } else if (warp == 10) {
@@ -408,7 +419,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int marks = 0;
 #pragma unroll 1
         for (int j = it.guard0; j < it.n_max; ++j, ++g) {
-          if (!mbar_wait_warp(&guard_full[g % kGuards], (g / kGuards) & 1, vabort)) {
+          if (!mbar_wait_warp(&guard_full[g % kGuards], (g / kGuards) & 1, waits)) {
             run = false;
             break;
           }
@@ -446,7 +457,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       row.reset();
 #pragma unroll 1
       for (int j = 0; j < it.n[s]; ++j, ++nt) {
-        if (!mbar_wait_warp(&s_full[s], nt & 1, vabort)) {
+        if (!mbar_wait_warp(&s_full[s], nt & 1, waits)) {
           run = false;
           break;
         }
@@ -470,7 +481,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tile::softmax_tile<HD>(lane_base, kColS + s * 128, kColO + s * 128, a.scale_log2, j == 0, masked, vis, row,
                                &p_half[2 * s], &p_half[2 * s + 1]);
       }
-      if (!run || !mbar_wait_warp(&o_full[s], no & 1, vabort)) break;
+      if (!run || !mbar_wait_warp(&o_full[s], no & 1, waits)) break;
       ++no;
       fence_after();
       const int marks = it.guard0 < it.n_max ? poison[item % kGuards] : 0;
@@ -509,7 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 
   __syncthreads();
-  if (*vabort) {
+  if (*waits.abort_flag) {
     if (tid == 0 && a.status) atomicOr(a.status, PSE_STATUS_TIMEOUT);
     if (tid == 0) {
       // copies still on their way land before the shared memory goes
@@ -641,6 +652,11 @@ extern "C" int pse_prompt_plan(const int32_t* lens, int32_t n, int32_t q_heads, 
   }
 }
 
+extern "C" int pse_attention_wait_tries(int32_t tries) {
+  t5::g_wait_tries.store(tries < 0 ? t5::kSpinLimit : (uint32_t)tries, std::memory_order_relaxed);
+  return PSE_OK;
+}
+
 extern "C" int pse_prompt_attention(const pse_head_view* views, int64_t tokens, int32_t head_dim, int32_t dtype,
                                     float scale, const int32_t* plan, int32_t n_cta, int64_t n_items, int32_t* status,
                                     void* stream) {
@@ -675,6 +691,7 @@ extern "C" int pse_prompt_attention(const pse_head_view* views, int64_t tokens, 
   a.n_cta = n_cta;
   a.n_items = (int)n_items;
   a.status = status;
+  a.wait_tries = t5::wait_tries();
   a.out_vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
   if (dtype == PSE_BF16 && prompt::tc_eligible(a))
     return head_dim == 64 ? prompt::launch_tc<64>(a, (cudaStream_t)stream)

@@ -12,6 +12,18 @@ namespace t5 {
 
 constexpr uint32_t kSpinLimit = 1u << 18;  // tries, a few microseconds each
 
+// The bound of a role's waits, and the flag by which the CTA's other roles learn
+// that one of them has expired.
+struct Waits {
+  volatile int* abort_flag;
+  uint32_t tries;
+};
+// The bound for the next launch's products: kSpinLimit, unless a test has set
+// another.  The other roles keep kSpinLimit in their code and give up with the
+// products (with a bound from the arguments in every wait, 64 short trees took 51.5 us
+// instead of 50.7).
+uint32_t wait_tries();
+
 __device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // ---------------------------------------------------------------- mbarriers
@@ -43,44 +55,44 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // suspends the thread in hardware for a while.  The loop is this short because
 // it stands in some thirty places: kernels whose warps walk different code
 // spend their time fetching it when it outgrows the instruction cache.)
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Waits& w) {
 #pragma unroll 1
-  for (uint32_t n = 0; n < kSpinLimit; ++n) {
+  for (uint32_t n = 0; n < w.tries; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
+    if (*w.abort_flag) return false;
   }
-  *abort_flag = 1;
+  *w.abort_flag = 1;
   return false;
 }
 // The same for a whole warp: every lane gets the same answer.  All lanes poll:
 // the warp has to arrive converged at the .aligned tensor-memory accesses that
 // follow, and a poll by one lane joined by a vote does not ensure that.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, const Waits& w) {
+  const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, w));
   __syncwarp();
   return ok;
 }
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return mbar_wait(su32(bar), parity, abort_flag);
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const Waits& w) {
+  return mbar_wait(su32(bar), parity, w);
 }
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return mbar_wait_warp(su32(bar), parity, abort_flag);
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, const Waits& w) {
+  return mbar_wait_warp(su32(bar), parity, w);
 }
 // Waits for three barriers at once (repeat one for fewer): their polls are on
 // their way together.
 __device__ __forceinline__ bool mbar_wait3_warp(uint32_t a, uint32_t pa, uint32_t b, uint32_t pb, uint32_t c, uint32_t pc,
-                                                volatile int* abort_flag) {
+                                                const Waits& w) {
   bool ok = false;
 #pragma unroll 1
-  for (uint32_t n = 0; n < kSpinLimit; ++n) {
+  for (uint32_t n = 0; n < w.tries; ++n) {
     const bool x = mbar_try_wait(a, pa), y = mbar_try_wait(b, pb), z = mbar_try_wait(c, pc);
     if (x && y && z) {
       ok = true;
       break;
     }
-    if (*abort_flag) break;
+    if (*w.abort_flag) break;
   }
-  if (!ok) *abort_flag = 1;
+  if (!ok) *w.abort_flag = 1;
   ok = __all_sync(0xffffffffu, ok);
   __syncwarp();
   return ok;

@@ -46,6 +46,7 @@ struct Args {
   int part_rows;
   int32_t* status;
   bool out_vec;  // output rows are 16-byte aligned
+  uint32_t wait_tries;  // of the products
 };
 
 // Partial results of cut items: per worker two blocks of `part_rows` rows, first
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   int* poison = abort_flag + 1;             // [kGuards] segments' marked tiles, bit j: tile g0 + j
   int* last_bar = poison + kGuards;         // [NS + 1] per slot (and Q): barrier and parity of its last copy
-  volatile int* vabort = abort_flag;
+  const Waits waits{abort_flag, kSpinLimit};
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
 #pragma unroll 1
     while (run && done < total) {
       // a segment is known here once its first scores stand
-      run = mbar_wait_warp(&s_full[s], done & 1, vabort);
+      run = mbar_wait_warp(&s_full[s], done & 1, waits);
       if (!run) break;
       const Seg& x = segs[items % kSegs];
       const int node = s * tpt + rt;  // within the block
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
 #pragma unroll
           for (int y = 0; y < 4; ++y) vis[y] = bits(t * 128 + 32 * y);
         }
-        if (t > t0) run = mbar_wait_warp(&s_full[s], done & 1, vabort);
+        if (t > t0) run = mbar_wait_warp(&s_full[s], done & 1, waits);
         if (!run) break;
         fence_after();
         if (!any_valid) {
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
           tile::softmax_tile<HD>(lane_base, s * 128, kColO + s * 128, a.scale_log2, t == t0, masked, vis, row,
                                  &p_half[2 * s], &p_half[2 * s + 1]);
       }
-      if (!run || !mbar_wait_warp(&o_full[s], items & 1, vabort)) break;
+      if (!run || !mbar_wait_warp(&o_full[s], items & 1, waits)) break;
       fence_after();
       const int marks = x.g0 < t1 ? poison[items % kGuards] : 0;
       const bool whole = t0 == 0 && t1 == x.tiles;
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
         }
         const uint32_t kbar = full0 + 8 * k;
         if (i < 0) {
-          run = mbar_wait3_warp(su32(q_full), segment & 1, kbar, kp, kbar, kp, vabort);
+          run = mbar_wait3_warp(su32(q_full), segment & 1, kbar, kp, kbar, kp, Waits{abort_flag, a.wait_tries});
           if (!run) break;
           const Seg& x = segs[segment++ % kSegs];
           nt = x.t1 - x.t0;
@@ -589,13 +590,13 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
           if (i >= 0) {
             const uint32_t part = part0 + 16 * s, par = parts >> s & 1u;
             // the output of the segment before has been read
-            if (i == 0) run = mbar_wait_warp(&o_empty[s], outs >> s & 1u, vabort);
-            run = run && (s == 0 ? mbar_wait3_warp(part, par, vbar, vp, kbar, kp, vabort)
-                                 : mbar_wait_warp(part, par, vabort));
+            if (i == 0) run = mbar_wait_warp(&o_empty[s], outs >> s & 1u, waits);
+            run = run && (s == 0 ? mbar_wait3_warp(part, par, vbar, vp, kbar, kp, waits)
+                                 : mbar_wait_warp(part, par, waits));
             if (!run) break;
             fence_after();
             issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 0, i == 0);
-            run = mbar_wait_warp(part + 8, par, vabort);
+            run = mbar_wait_warp(part + 8, par, waits);
             if (!run) break;
             fence_after();
             issue_values<HD>(el, o_col, s_col, ring0 + v * kTileBytes, 1, false);
@@ -657,7 +658,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
           for (int p = 0; p < 8; ++p) y[p] = __shfl_sync(0xffffffffu, cur, (src + p) & 31);
 #pragma unroll 1
           for (int kv = kv0; kv <= kv1; ++kv) {
-            run = mbar_wait_warp(empty0 + 8 * slot, fill ^ 1, vabort);
+            run = mbar_wait_warp(empty0 + 8 * slot, fill ^ 1, waits);
             if (!run) break;
             const bool guarded = kv == 1 && t >= g0;
             const uint32_t bar = guarded ? guard0 + 8 * (gd % kGuards) : full0 + 8 * slot;
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
         int n = 0;
 #pragma unroll 1
         while (walk.next(g)) {
-          if (!mbar_wait(q_empty, (n & 1) ^ 1, vabort)) break;
+          if (!mbar_wait(q_empty, (n & 1) ^ 1, waits)) break;
           // (the segment kSegs before has been written out: the one before this
           // has made its last scores, which came after its own first product,
           // and that after the reading of the output before it)
@@ -726,7 +727,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
         int marks = 0;
 #pragma unroll 1
         for (int t = g0; t < g.t1; ++t, ++gd) {
-          run = mbar_wait_warp(&guard_full[gd % kGuards], (gd / kGuards) & 1, vabort);
+          run = mbar_wait_warp(&guard_full[gd % kGuards], (gd / kGuards) & 1, waits);
           if (!run) break;
           const int s = (2 * (tiles + t - g.t0) + 1) % NS;
           if (tile::clear_nonfinite(reinterpret_cast<uint4*>(ring + s * kTileBytes), kTileBytes / 16))
@@ -743,7 +744,7 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
   }
 
   __syncthreads();
-  if (*vabort && tid == 0) {
+  if (*waits.abort_flag && tid == 0) {
     atomicOr(a.status, PSE_STATUS_TIMEOUT);
     for (int i = 0; i < NS; ++i)
       if (last_bar[i] >= 0) {
@@ -907,6 +908,7 @@ extern "C" int pse_token_tree_attention(pse_block_state st, pse_kv_layer kv, con
   a.cuts = (tree::Cut*)workspace;
   a.parts = (float*)((char*)workspace + tree::kCutBytes);
   a.status = st.status;
+  a.wait_tries = t5::wait_tries();
   a.out_vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
   if (kv.dtype == PSE_BF16 && tree::tc_eligible(a, q.heads))
     return a.hd == 64 ? tree::tc_attention<64>(a, q.heads, max_nodes, (cudaStream_t)stream)

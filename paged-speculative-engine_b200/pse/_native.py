@@ -97,6 +97,7 @@ _PROTOS = {
     "pse_rotary_append": ([BlockState, KVLayer, RotarySpec, c_p, c_p, c_p, c_p, c_i64, c_p], 1),
     "pse_prompt_plan": ([c_p, c_i32, c_i32, c_i32, c_i32, c_p, c_i64, c_p], 0),
     "pse_prompt_attention": ([c_p, c_i64, c_i32, c_i32, c_f32, c_p, c_i32, c_i64, c_p, c_p], 1),
+    "pse_attention_wait_tries": ([c_i32], 0),
     "pse_tree_masks": ([c_p, c_p, c_i32, c_i32, c_i32, c_p, c_p, c_p], 1),
     "pse_token_tree_attention": ([BlockState, KVLayer, c_p, c_p, c_p, c_p, c_i32, c_i32, c_i32, c_p, c_i32, c_f32,
                                   c_p, c_sz, c_p], 2),
