@@ -295,8 +295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           return true;
         };
 #pragma unroll 1
-#pragma unroll 1
-    for (int e = e0; run && e < e1; ++e) {
+        for (int e = e0; run && e < e1; ++e) {
           const TcItem it = decode(a, e, tpt);
           if (it.n_max == 0) continue;
 #pragma unroll 1
@@ -329,7 +328,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // -------------------------------------------------------------- products
       const uint32_t el = elect_one();
       const Waits tries{abort_flag, a.wait_tries};
-      const uint32_t full0 = su32(slot_full), empty0 = su32(slot_empty), ring0 = su32(ring), q0 = su32(q_s);
+      const uint32_t full0 = su32(slot_full), ring0 = su32(ring), q0 = su32(q_s);
       const uint32_t part0 = su32(p_half);
       int slot = 0;
       uint32_t fill = 0;
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       };
 #pragma unroll 1
-    for (int e = e0; run && e < e1; ++e) {
+      for (int e = e0; run && e < e1; ++e) {
         const TcItem it = decode(a, e, tpt);
         if (it.n_max == 0) continue;
         const int n0 = it.n[0], n1 = it.n[1], n = it.n_max;
@@ -413,7 +412,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int c = 0, g = 0, items = 0;
       bool run = true;
 #pragma unroll 1
-    for (int e = e0; run && e < e1; ++e) {
+      for (int e = e0; run && e < e1; ++e) {
         const TcItem it = decode(a, e, tpt);
         if (it.n_max == 0) continue;
         int marks = 0;
@@ -542,16 +541,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 Map3Cache g_maps;
 
-bool tc_view(const char* p, int64_t tok, int64_t head, int heads, int hd) {
-  if (heads == 1) head = hd;  // the stride of an axis of one is not used
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= hd && head >= hd &&
-         tok < (1ll << 38) && head < (1ll << 38);
-}
-
 bool tc_eligible(const Args& a) {
   return (a.hd == 64 || a.hd == 128) && a.group <= 128 && a.scale_log2 > 0.f &&
-         tc_view(a.q, a.q_tok, a.q_head, a.q_heads, a.hd) && tc_view(a.k, a.k_tok, a.k_head, a.kv_heads, a.hd) &&
-         tc_view(a.v, a.v_tok, a.v_head, a.kv_heads, a.hd);
+         tma_rows(a.q, a.q_tok, a.q_head, a.q_heads, a.hd) && tma_rows(a.k, a.k_tok, a.k_head, a.kv_heads, a.hd) &&
+         tma_rows(a.v, a.v_tok, a.v_head, a.kv_heads, a.hd);
 }
 
 template <int HD>

@@ -110,12 +110,6 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) { mba
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(su32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(su32(bar))
-      : "memory");
-}
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -123,7 +117,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// The same from a converged warp, issued by its elected lane (see mma_ss below).
+// From a converged warp, issued by its elected lane (see mma_ss below).
 __device__ __forceinline__ void tma_load_2d(uint32_t elected, uint32_t dst, const CUtensorMap* map, int x, int y,
                                             uint32_t bar) {
   asm volatile(
@@ -132,6 +126,13 @@ __device__ __forceinline__ void tma_load_2d(uint32_t elected, uint32_t dst, cons
       "[%4];\n}\n" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(elected)
       : "memory");
+}
+
+// Whether a [tokens, heads, hd] bf16 view can be read through a 3-D tensor map.
+inline bool tma_rows(const char* p, int64_t tok, int64_t head, int heads, int hd) {
+  if (heads == 1) head = hd;  // the stride of an axis of one is not used
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= hd && head >= hd &&
+         tok < (1ll << 38) && head < (1ll << 38);
 }
 
 // ---------------------------------------------------------------- tensor cores

@@ -764,18 +764,12 @@ __global__ void __launch_bounds__(n_threads<NQ>(), NQ == 1 ? 2 : 1)
 Map3Cache g_q_maps;
 TmapCache g_pool_maps;
 
-bool tc_rows(const char* p, int64_t tok, int64_t head, int heads, int hd) {
-  if (heads == 1) head = hd;  // the stride of an axis of one is not used
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && tok % 8 == 0 && head % 8 == 0 && tok >= hd && head >= hd &&
-         tok < (1ll << 38) && head < (1ll << 38);
-}
-
 bool tc_eligible(const Args& a, int q_heads) {
   const int64_t pool_rows = (int64_t)a.num_blocks * a.rows.kv_heads * a.block_size;
   return (a.hd == 64 || a.hd == 128) &&
          (a.block_size == 16 || a.block_size == 32 || a.block_size == 64 || a.block_size == 128) && a.num_blocks > 0 &&
          a.scale_log2 > 0.f && (reinterpret_cast<uintptr_t>(a.k_pool) | reinterpret_cast<uintptr_t>(a.v_pool)) % 16 == 0 &&
-         pool_rows + a.block_size < (1ll << 31) && tc_rows(a.q, a.q_tok, a.q_head, q_heads, a.hd);
+         pool_rows + a.block_size < (1ll << 31) && tma_rows(a.q, a.q_tok, a.q_head, q_heads, a.hd);
 }
 
 template <int HD, int NQ>

@@ -43,11 +43,6 @@ class TokenTrees:
         self.fn = N.fn("pse_token_tree_attention")
         self._masks_ptr = masks.data_ptr()
 
-    @classmethod
-    def from_parents(cls, parents: torch.Tensor, counts) -> "TokenTrees":
-        """The trees of packed ``parents`` (see ``tree_masks``); ``depths`` is set."""
-        return tree_masks(parents, counts)
-
 
 def _offsets(counts, device) -> torch.Tensor:
     out = [0]
