@@ -136,11 +136,12 @@ def written_view(name: str, t: torch.Tensor, tokens: int, heads: int, head_dim: 
     """``head_view`` of a tensor that the kernel writes, whose elements must each
     have a place of their own."""
     view = head_view(name, t, tokens, heads, head_dim, dtype, device)
-    reach = head_dim
-    for stride, n in sorted(((view[1], tokens), (view[2], heads))):
-        if n > 1 and stride < reach and tokens and heads:
-            raise ValueError(f"{name} overlaps itself (strides {t.stride()})")
-        reach += max(n - 1, 0) * stride
+    if not t.is_contiguous():
+        reach = head_dim
+        for stride, n in sorted(((view[1], tokens), (view[2], heads))):
+            if n > 1 and stride < reach and tokens and heads:
+                raise ValueError(f"{name} overlaps itself (strides {t.stride()})")
+            reach += max(n - 1, 0) * stride
     return view
 
 
