@@ -8,7 +8,9 @@
 // 128 / group tokens each, the group's heads side by side in a tile; the items
 // are dealt to the CTAs longest first, each to the CTA with the least work so
 // far, which needs no counter on the device and gives the same order of
-// operations in every call.
+// operations in every call.  (The CUDA-core kernel has a block per 64 rows of an
+// item instead; its blocks start in the list's order, one CTA's items after the
+// other's, not the longest first.)
 #include <algorithm>
 #include <atomic>
 #include <queue>
@@ -155,15 +157,20 @@ int simt_attention(const Args& a, cudaStream_t s) {
 //   warp 11         TMA: Q tiles, so that the ring runs on into the next item
 // While a stream's softmax runs, the tensor cores work on the other stream.
 //
-// Measured: 8192-token prompts, 32 + 8 heads of 128: 1250 TFLOP/s; three prompts
-// of 5003 to 8192 tokens 893 us, 1208 TFLOP/s of the 1660 that a large matrix product
-// reaches: what is lost are the hand-overs between the softmax warps and the
-// products (each some 200 clocks of a tile's 2800) and the work beyond the diagonal.
-// Heads of 64 need twice the exponentials per product and are bound by them: 2048
-// token prompts 598 TFLOP/s; 24 prompts of 17 to 1500 tokens 72 us.  One prompt of 37
-// tokens 5.3 us, all of it latency.  Tried and slower: a third of the exponentials
-// by a polynomial on the FMA units, 96 + 32 keys instead of 64 + 64 to a hand-over,
-// a warp per stream for the products, weights apart from the scores.
+// Measured: three prompts of 5003 to 8192 tokens, 32 + 8 heads of 128: 900 us in
+// bursts of 20 calls at full clock, 1200 TFLOP/s of the 1660 that a large matrix
+// product reaches so; 1048 us and 1030 TFLOP/s of 1370 in a loop of calls, where the
+// power cap holds the clock.  What is lost are the hand-overs between the softmax
+// warps and the products (each some 200 clocks of a tile's 2800) and the work beyond
+// the diagonal.  Heads of 64 need twice the exponentials per product: 2048 token
+// prompts 640 TFLOP/s (600 in a loop), the exponential pipe 61% busy.  24 prompts of
+// 17 to 1500 tokens, heads of 64, take 71 us: 8 or 9 items to a CTA with 31 us of
+// exponentials, the rest hand-overs and items' beginnings and ends (an item's queries
+// are loaded when the scores of the item before have retired, and its first softmax
+// waits for them).  One prompt of 37 tokens 5.1 us, all of it latency.
+// Tried and slower: a third of the exponentials by a polynomial on the FMA units,
+// 96 + 32 keys instead of 64 + 64 to a hand-over, a warp per stream for the products,
+// weights apart from the scores.
 //
 // A hidden key has weight zero, but 0 x inf is NaN in a product, and a tile at
 // the causal edge or the prompt's end holds V rows of later tokens or of the

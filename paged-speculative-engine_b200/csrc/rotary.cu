@@ -9,7 +9,8 @@
 // one unit of a head, two 16-byte vectors (V pairs), for kHeads heads of one
 // token, and issues all its loads first; while they are in flight the block
 // computes its tokens' sines and cosines, each once, into shared memory (105 us
-// where each thread computed its own, 62 so, at the size below: 5.4 TB/s).  The
+// where each thread computed its own, 62 so, at the size below: 5.4 TB/s; 65 and
+// 5.1 where every call has other inputs).  The
 // angle is kept in turns and reduced in fp64 (one multiply, one rounding, one
 // subtraction), so the fp32 sine and cosine are those of the exact angle at any
 // int32 position; no table is read.
@@ -19,9 +20,9 @@ namespace pse {
 namespace {
 
 // Heads of a token whose loads a thread has in flight together.  Two, with
-// registers held to 48 (56 with the append) so that 1100 threads stay resident:
-// 61.9 us at 16384 tokens, 32 + 8 heads of 128 in bf16, against 81.4 with four
-// heads at 96 registers and 74.4 with one.
+// registers held to 48, so that 1280 threads stay resident (64 with the append, and
+// 1024): 61.9 us at 16384 tokens, 32 + 8 heads of 128 in bf16, against 81.4 with
+// four heads at 96 registers and 74.4 with one.
 constexpr int kHeads = 2;
 
 struct View {

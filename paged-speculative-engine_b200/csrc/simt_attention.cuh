@@ -9,10 +9,13 @@
 // by 4 floats (16 lanes reading 16 rows' vectors touch every bank once per
 // quarter warp).  One pass over the keys with a running maximum and sum.
 //
-// Bound by the instructions of 8 warps that hide little of each other's latency:
-// products in pairs of columns (two fp32 results an instruction), a tile's loads
+// Products in pairs of columns (two fp32 results an instruction), a tile's loads
 // together, masks as bits per row.  8 prompts of 1000 tokens, 12 heads of 64: 480
-// us, 26 TFLOP/s (1080 us and 11 with 16 query rows per block instead of 64).
+// us, 26 TFLOP/s (1080 us and 11 with 16 query rows per block instead of 64); bound
+// by the instructions of the two blocks, 16 warps, that a multiprocessor holds (2.3
+// a clock), and by a tile's loads, which nothing is multiplied under.  Few short
+// prompts leave a block alone on its multiprocessor, its 8 warps waiting in turn for
+// each tile's loads and for each other: the five tiles of 300 tokens take 37 to 47 us.
 #pragma once
 
 #include "tcgen05.cuh"

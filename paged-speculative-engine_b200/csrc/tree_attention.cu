@@ -5,15 +5,16 @@
 // bits, one word per 64 nodes, and rows may hold different numbers of nodes.
 //
 // The context's K/V is read from HBM once per request, which bounds the call
-// until a K/V head has about 256 query rows (nodes x group).  Measured: 16
-// requests of 16384 tokens, 8 K/V heads of 128: 8 nodes (32 rows) 178 us (6.0
-// TB/s, 92% of a copy's rate), 32 nodes (128 rows) 197 us, 64 nodes (256 rows) 277
-// us (990 TFLOP/s, the products and the softmax in turn).  At head_dim 64 a row of
-// scores costs twice as many exponentials for its bytes, and the softmax warps
-// bound the call: 64 requests of 2048 tokens with 26 nodes 85 us (3.4 TB/s), with 6
-// nodes 66 us (4.1 TB/s).  A small tree (8 nodes, 300 tokens) takes 11 us, of which
-// 5 pass before the first scores stand (launch, the split of the work, the first
-// loads) and 3 in the join.
+// until a K/V head has about 256 query rows (nodes x group).  Measured, in bursts of
+// 20 calls (and in a loop of calls, where the power cap holds the clock): 16
+// requests of 16384 tokens, 8 K/V heads of 128: 8 nodes (32 rows) 177 us (201), 6.1
+// TB/s, 93% of a copy's rate; 32 nodes (128 rows) 194 us (223); 64 nodes (256 rows)
+// 271 us (326), 1014 TFLOP/s, the products and the softmax in turn.  At head_dim 64 a
+// row of scores costs twice as many exponentials for its bytes, and the softmax
+// warps bound the call: 64 requests of 2048 tokens with 26 nodes 85 us (89), 3.4
+// TB/s; with 6 nodes 68 us (72), 4.0 TB/s.  A small tree (8 nodes, 300 tokens) takes
+// 11 us, of which 5 pass before the first scores stand (launch, the split of the
+// work, the first loads) and 3 in the join: the split leaves no item whole there.
 #include "attention_tile.cuh"
 #include "simt_attention.cuh"
 #include "tmap_cache.h"
@@ -274,9 +275,10 @@ __global__ void __launch_bounds__(simt::kThreads) tree_simt_kernel(const Args a)
   if (threadIdx.x == 0) *reinterpret_cast<int4*>(a.cuts + blockIdx.x) = make_int4(cut.last, cut.node0, cut.nodes, cut.hk);
 }
 
-// Rows per thread: blocks of 16 query rows up to 32, of 64 above (26 rows: 52
-// against 63 us, 104 rows: 684 against 413 us; 8 requests of 500 tokens and 12 K/V
-// heads, 16 of 2000 and 8).
+// Rows per thread: blocks of 16 query rows up to 32, of 64 above.  16 against 64, 8
+// requests of 500 tokens and 12 K/V heads: 26 rows 51 and 63 us, 33 rows 70 and 62,
+// 48 rows 71 and 64, 63 rows 94 and 69; 16 requests of 2000 tokens and 8 K/V heads: 24
+// rows 206 and 218 us, 40 rows 301 and 219, 56 rows 400 and 221, 104 rows 684 and 413.
 int simt_rows(int rows, int group) { return rows <= 32 && group <= 16 ? 1 : 4; }
 
 template <typename T, int RPT, int NC>

@@ -16,7 +16,8 @@ from .rotary import head_view, new_result, written_view
 class PackedPrompts:
     """The packing of one batch of prompts: ``lengths`` tokens each, one after
     the other, and the attention's work list for it (built on the host, one
-    copy to the device).  One object serves every layer of a forward and any
+    copy to the device: 0.1 ms for 24 prompts of up to 1500 tokens, 2.4 ms for
+    32 of 8192, 32 + 8 heads).  One object serves every layer of a forward and any
     number of calls, made with its device current; it is not changed by them,
     except for ``status``, where a kernel leaves an error (``check_status``)."""
 
@@ -71,7 +72,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prompts:
     any token and head strides (views of a fused projection included); T is
     the packing's total.  ``scale`` defaults to 1 / sqrt(head_dim).  Returns
     [T, q_heads, head_dim] (``out`` if given, which must not overlap the
-    inputs)."""
+    inputs), without a gradient.
+
+    bfloat16 with a head_dim of 64 or 128, at most 128 query heads to a K/V
+    head, a positive scale, and q, k, v whose base and strides are multiples of
+    16 bytes and whose heads and tokens lie apart runs on the tensor cores.
+    Anything else runs in fp32 on the CUDA cores, at some 26 TFLOP/s instead
+    of 600 to 1200."""
     shape, dtype, dev = getattr(q, "shape", ()), getattr(q, "dtype", None), prompts.index
     stream = N.stream_on(dev)
     hd = shape[2] if len(shape) == 3 else 0

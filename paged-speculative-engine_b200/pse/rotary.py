@@ -3,7 +3,8 @@ long contexts, with or without the append into a paged cache.
 
 The engine's own forward (``pse.engine``) keeps its in-place rotate-half
 kernel; these entry points serve models whose positions differ from it, and
-calls packed over requests of different lengths.
+calls packed over requests of different lengths.  They serve: results carry no
+gradient, whatever the inputs require.
 """
 from __future__ import annotations
 

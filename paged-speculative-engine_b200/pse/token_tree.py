@@ -94,7 +94,13 @@ def token_tree_attention(q: torch.Tensor, cache, layer: int, slots: torch.Tensor
     head_dim] in the cache's dtype, any token and head strides; ``slots`` int32
     [rows] (``cache.slots_tensor``).  The nodes' K/V must be in the cache, node
     j at position context + j.  ``scale`` defaults to 1 / sqrt(head_dim).
-    Returns [nodes, q_heads, head_dim]; a node that sees nothing gives zeros."""
+    Returns [nodes, q_heads, head_dim], without a gradient; a node that sees
+    nothing gives zeros.
+
+    A bfloat16 cache with a head_dim of 64 or 128 and pages of 16, 32, 64 or 128
+    tokens, a positive scale, and q whose base and strides are multiples of 16
+    bytes runs on the tensor cores.  Anything else runs in fp32 on the CUDA
+    cores, many times slower where there are more than a few nodes."""
     hd, dtype, dev = cache.head_dim, cache.dtype, trees.index
     stream = N.stream_on(dev)
     if cache.device.index != dev:
