@@ -145,10 +145,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a, int wo
       for (int i = 0; i < 4; ++i) {
         if (i0 + i >= n) break;
         const float f = exp2f(ml[i].x - ms);
-        L += ml[i].y * f;  // a sum is finite or the NaN of a score
+        // (a part that saw nothing is all zeros; an infinity or NaN that a row sees
+        // reaches it from the smallest part too)
+        L += ml[i].y * f;
         const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
 #pragma unroll
-        for (int d = 0; d < 8; ++d) acc[d] += f == 0.f ? 0.f : v[d] * f;
+        for (int d = 0; d < 8; ++d) acc[d] = fmaf(v[d], f, acc[d]);
       }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;

@@ -312,3 +312,23 @@ def test_refusals_of_kept_buffers():
 def test_few_rows_of_large_groups(group, nodes):
     """The CUDA-core kernel's blocks hold whole groups, and any number of rows around its two sizes."""
     Case([70] * len(nodes), nodes, 2 * group, 2, 40, 8, torch.float32, group).check()
+
+
+@pytest.mark.parametrize("hd,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float32), (80, torch.bfloat16)])
+def test_a_visible_infinity_of_no_weight_reaches_the_row(hd, dtype):
+    """A key that a row sees counts, however far its score lies below the
+    largest: 0 x inf is NaN, wherever the work is cut."""
+    ctx = 3000
+    c = Case([ctx], [3], 2, 2, hd, 16, dtype, 2)
+    c.cache.truncate("r0", 0)
+    c.q.fill_(1.0)
+    c.k[0].zero_()
+    c.k[0][:, ctx] = 400.0 / math.sqrt(hd)  # the first node, an ancestor of all: scores of 400
+    c.visible[:, 0] = True
+    c.trees = __import__("pse").TokenTrees(words(c.visible).cuda(), [3])
+    c.v[0][0, 5, 1], c.v[0][1, 7, 2] = math.nan, math.inf
+    c.fill()
+    got = c.run()
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[:, 0, 1] = bad[:, 1, 2] = True
+    assert not torch.isfinite(got[bad]).any() and torch.isfinite(got[~bad]).all()
