@@ -174,8 +174,9 @@ struct Tile {
         unpack2(s2[i][j], s[j], odd);
         s[j] += odd;
       }
+      uint64_t vis = ~0ull;
       if (masked) {
-        const uint64_t vis = visible(i) >> tx;
+        vis = visible(i) >> tx;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (!(vis >> (16 * j) & 1ull)) s[j] = -INFINITY;
@@ -196,7 +197,8 @@ struct Tile {
       for (int j = 0; j < 4; ++j) {
         const float w = exp2f(s[j] - ms);
         l[i] += w;
-        p[(ty * RPT + i) * (BK + 4) + tx + 16 * j] = w;
+        // (a hidden key's zero is negative: a seen key's weight may underflow)
+        p[(ty * RPT + i) * (BK + 4) + tx + 16 * j] = masked && !(vis >> (16 * j) & 1ull) ? -0.f : w;
       }
     }
     __syncwarp();  // a row's weights are written and read by one half warp
@@ -206,8 +208,8 @@ struct Tile {
       values<false>();
   }
   // o += p v.  Columns past the head's are computed and not used (their reads end
-  // inside the tile's memory).  MASKED: a weight of zero takes no part, which
-  // matters where V is infinite or NaN.
+  // inside the tile's memory).  MASKED: a hidden key's weight (-0) takes no part,
+  // which matters where V is infinite or NaN.
   template <bool MASKED>
   __device__ __forceinline__ void values() {
 #pragma unroll 4
@@ -230,7 +232,7 @@ struct Tile {
 #pragma unroll
           for (int i = 0; i < RPT; ++i) {
             const float y = x == 0 ? w[i].x : x == 1 ? w[i].y : x == 2 ? w[i].z : w[i].w;
-            if (skip && y == 0.f) continue;
+            if (skip && __float_as_uint(y) == 0x80000000u) continue;
             o[i][c][0] = fma2(pack2(y, y), b.x, o[i][c][0]);
             o[i][c][1] = fma2(pack2(y, y), b.y, o[i][c][1]);
           }

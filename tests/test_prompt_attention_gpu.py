@@ -232,3 +232,19 @@ def test_many_short_items_behind_a_long_one(hd):
         t += n
     got = run(q, k, v, lens)
     assert bool((got[seen] == math.inf).all()) and torch.equal(got[~seen], clean[~seen])
+
+
+@pytest.mark.parametrize("hd,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float32), (80, torch.bfloat16)])
+def test_a_visible_infinity_of_no_weight_reaches_the_row(hd, dtype):
+    """A key that a token sees counts, however far its score lies below the largest: 0 x inf is NaN."""
+    lens = [200, 30]
+    q, k, v = (x.clone() for x in inputs(lens, 2, 2, hd, dtype, 2))
+    q.fill_(1.0)
+    k.zero_()
+    k[0] = k[200] = 400.0 / math.sqrt(hd)  # scores of 400 beside zeros
+    seen = torch.zeros_like(q, dtype=torch.bool)
+    for t, h, d in ((5, 0, 1), (150, 1, 2), (210, 0, 3)):
+        v[t, h, d] = math.inf if t == 150 else math.nan
+        seen[t:200 if t < 200 else 230, h, d] = True
+    got = run(q, k, v, lens)
+    assert not torch.isfinite(got[seen]).any() and torch.isfinite(got[~seen]).all()

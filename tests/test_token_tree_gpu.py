@@ -332,3 +332,21 @@ def test_a_visible_infinity_of_no_weight_reaches_the_row(hd, dtype):
     bad = torch.zeros_like(got, dtype=torch.bool)
     bad[:, 0, 1] = bad[:, 1, 2] = True
     assert not torch.isfinite(got[bad]).any() and torch.isfinite(got[~bad]).all()
+
+
+@pytest.mark.parametrize("hd,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float32), (80, torch.bfloat16)])
+@pytest.mark.parametrize("at", [5, 41])
+def test_an_infinity_of_no_weight_in_a_tile_with_a_mask(at, hd, dtype):
+    """The same beside hidden keys: in the context, and in a node that the next ones see and the one before does not."""
+    c = Case([40], [4], 2, 2, hd, 16, dtype, 2, visible=ancestor_rows([-1, -1, 1, 2], 64))
+    c.cache.truncate("r0", 0)
+    c.q.fill_(1.0)
+    c.k[0].zero_()
+    c.k[0][:, 7] = 400.0 / math.sqrt(hd)  # a key of the context, which all see
+    c.v[0][0, at, 1], c.v[0][1, at, 2] = math.nan, math.inf
+    c.fill()
+    got = c.run()
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    first = 0 if at < 40 else 1
+    bad[first:, 0, 1] = bad[first:, 1, 2] = True
+    assert not torch.isfinite(got[bad]).any() and torch.isfinite(got[~bad]).all()
